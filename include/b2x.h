@@ -334,6 +334,183 @@ B2X_API b2x_status b2x_fp8_grouped_gemm(const b2x_gemm_group* groups, int num_gr
                                         b2x_dtype b_type, b2x_dtype c_type, int block_n, void* workspace,
                                         size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------ GEMM with epilogue */
+
+typedef enum {
+  B2X_ACT_NONE = 0,
+  B2X_ACT_RELU = 1,
+  B2X_ACT_GELU = 2,      /* x erfc(-x / sqrt 2) / 2 */
+  B2X_ACT_GELU_TANH = 3, /* x sigmoid(2 sqrt(2/pi) (x + 0.044715 x^3)) */
+  B2X_ACT_SILU = 4
+} b2x_activation;
+
+/*
+ * What follows the product in b2x_fp8_gemm_epilogue:
+ *   pre = A . B * scales + bias        (fp32)
+ *   C   = act(pre) + residual          (fp32, rounded once to c_type)
+ * bias [N] (fp32, bf16 or fp16; NULL: none), residual [M, N] of c_type (row
+ * stride ld_residual; NULL: none), pre [M, N] of c_type (row stride ld_pre;
+ * NULL: not stored), what b2x_epilogue_backward takes.  residual may be c.
+ */
+typedef struct {
+  const void* bias;
+  b2x_dtype bias_type;
+  b2x_activation activation;
+  const void* residual;
+  int64_t ld_residual;
+  void* pre;
+  int64_t ld_pre;
+} b2x_epilogue;
+
+/*
+ * C = act(A . B * scales + bias) + residual for the arguments of b2x_fp8_gemm
+ * with per-tensor scales or none (config is ignored; no workspace).  Sums over
+ * K are reduced in a fixed order: the same inputs give the same bits.
+ */
+B2X_API b2x_status b2x_fp8_gemm_epilogue(const b2x_gemm_args* args, const b2x_epilogue* ep, void* stream);
+
+/*
+ * Backward of that epilogue: d_pre = grad * act'(pre) [rows, cols] of `type`
+ * (bf16, fp16 or fp32; unit column strides) and, if d_bias is not NULL,
+ * d_bias[n] = sum over rows of the unrounded d_pre (fp32, fixed order).  The
+ * residual's gradient is grad itself.  d_pre may be grad or pre.
+ */
+B2X_API b2x_status b2x_epilogue_backward(const void* grad, int64_t ld_grad, const void* pre, int64_t ld_pre,
+                                         void* d_pre, int64_t ld_d_pre, float* d_bias, b2x_dtype type, int64_t rows,
+                                         int64_t cols, b2x_activation activation, void* stream);
+
+/* ------------------------------------------------------------ mixture of experts */
+
+/*
+ * Routing.  For each of `tokens` rows of logits [tokens, experts] (fp32, bf16
+ * or fp16, unit column stride):
+ *   s      = softmax(l) or sigmoid(l)
+ *   choice = s + bias                                  (bias [experts] fp32 or NULL)
+ *   groups: the experts in num_groups equal runs; a group scores the largest
+ *           (group_top2 = 0) or the sum of its two largest choices; only the
+ *           experts of the top_groups best groups stay
+ *   the top_k largest choices, in falling order, are the row's experts, and
+ *   weight = s of each, divided by their sum if renormalize, times scale.
+ * Choices are compared as exactly as fp64 gives them; equal ones go to the
+ * lower index.  An expert whose logit or bias is -inf is masked: it is never
+ * chosen and weighs nothing; where fewer than top_k experts are left, the
+ * remaining slots hold expert -1 and weight 0.  NaN ranks above all numbers
+ * and its weight is NaN.  experts <= 1024, top_k <= 32.
+ */
+typedef struct {
+  const void* logits;
+  b2x_dtype logits_type;
+  int64_t tokens, experts, ld_logits;
+  int top_k;
+  int sigmoid; /* 0 softmax, 1 sigmoid */
+  const float* bias;
+  int num_groups, top_groups, group_top2;
+  int renormalize;
+  float scale;
+  float* weights;   /* [tokens, top_k] */
+  int32_t* indices; /* [tokens, top_k] */
+} b2x_moe_route_args;
+
+B2X_API b2x_status b2x_moe_route(const b2x_moe_route_args* args, void* stream);
+
+/*
+ * Gradient of the routing weights: d_logits [tokens, experts] (row stride
+ * ld_d_logits, logits_type) from d_weights [tokens, top_k] and the forward's
+ * logits and indices (args->weights, bias and the group fields are not read).
+ * The choice itself has no gradient.  Indices outside [0, experts) count as
+ * empty slots.
+ */
+B2X_API b2x_status b2x_moe_route_backward(const b2x_moe_route_args* args, const float* d_weights, void* d_logits,
+                                          int64_t ld_d_logits, void* stream);
+
+/*
+ * Dispatch: the (token, slot) pairs of indices [tokens, top_k], stably sorted
+ * by expert.  offsets [experts + 1] receives where each expert's rows start,
+ * rows [tokens, top_k] the row of each pair (-1 for an index outside
+ * [0, experts): the pair is dropped), and row r of q [tokens * top_k, cols]
+ * (row stride ld_q) the token's x in fp8 with the recipe of b2x_fp8_cast:
+ * one scale per row, s = amax / FMAX, written to scale[r], or, with `given`
+ * not NULL, that one scale for all (then scale is not written).  Rows from
+ * offsets[experts] on are left as they were.  x is fp32 or bf16.
+ */
+typedef struct {
+  const void* x;
+  b2x_dtype x_type;
+  int64_t tokens, cols, ld_x;
+  const int32_t* indices;
+  int top_k;
+  int64_t experts;
+  void* q;
+  b2x_dtype q_type;
+  int64_t ld_q;
+  float* scale;
+  const float* given;
+  int32_t* offsets;
+  int32_t* rows;
+} b2x_moe_dispatch_args;
+
+B2X_API b2x_status b2x_moe_dispatch(const b2x_moe_dispatch_args* args, void* stream);
+
+/*
+ * The experts' products over rows sorted by expert, with the row ranges on
+ * the device: for r in [offsets[e], offsets[e + 1])
+ *   y[r, n] = scale_x[r] * scale_w[e] * sum_k x[r, k] w[e, n, k].
+ * x: fp8 [rows, K] (row stride ld_x).  w: fp8, element (e, n, k) at
+ * e * ldw_e + n * ldw_n + k * ldw_k with ldw_k or ldw_n equal to 1.  scale_x:
+ * fp32, one (scale_x_count = 1) or one per row; scale_w: one or one per
+ * expert; NULL for 1.  offsets must rise from 0 to at most rows; rows from
+ * offsets[experts] on are left as they were.  No host copy of the sizes is
+ * needed, no workspace, and the call can be captured into a CUDA graph.
+ */
+typedef struct {
+  const void* x;
+  b2x_dtype x_type;
+  int64_t rows, K, ld_x;
+  const void* w;
+  b2x_dtype w_type;
+  int64_t experts, N, ldw_e, ldw_n, ldw_k;
+  const int32_t* offsets;
+  const float* scale_x;
+  int64_t scale_x_count;
+  const float* scale_w;
+  int64_t scale_w_count;
+} b2x_moe_gemm_args;
+
+B2X_API b2x_status b2x_moe_gemm(const b2x_moe_gemm_args* args, void* y, b2x_dtype y_type, int64_t ld_y, void* stream);
+
+/*
+ * The same with SwiGLU and fp8 in the epilogue: w[e] is the K-major [2I, K]
+ * gate and up weight in alternating blocks of 128 rows (as for
+ * b2x_fp8_gemm_swiglu), N = 2I a multiple of 256, ldw_e = N * ldw_n, and
+ *   h[r, i] = fp8(silu(g) * u / *h_scale)     [rows, I], row stride ld_h.
+ * If h_amax is not NULL, max |silu(g) u| is max-reduced into it.
+ */
+B2X_API b2x_status b2x_moe_gemm_swiglu(const b2x_moe_gemm_args* args, void* h, b2x_dtype h_type, int64_t ld_h,
+                                       const float* h_scale, float* h_amax, void* stream);
+
+/*
+ * Combine: out[t] = sum_j weights[t, j] * y[rows[t, j]] + residual[t], summed
+ * in fp32 in the order of j and rounded once.  y [y_rows, cols] (row stride
+ * ld_y) and out, residual [tokens, cols] are of `type` (bf16, fp16 or fp32).
+ * weights [tokens, top_k] fp32, NULL: all 1 (the backward pass of the
+ * dispatch's gather).  Rows outside [0, y_rows) are dropped pairs.
+ */
+B2X_API b2x_status b2x_moe_combine(const void* y, int64_t y_rows, int64_t ld_y, const int32_t* rows,
+                                   const float* weights, int64_t tokens, int top_k, int64_t cols,
+                                   const void* residual, int64_t ld_residual, void* out, int64_t ld_out,
+                                   b2x_dtype type, void* stream);
+
+/*
+ * Its gradients: d_y[rows[t, j]] = weights[t, j] * grad[t] and
+ * d_weights[t, j] = <grad[t], y[rows[t, j]]> (fp32, fixed order; 0 for a
+ * dropped pair).  The residual's gradient is grad.  Rows of d_y that no pair
+ * names are left as they were; a row is named at most once.
+ */
+B2X_API b2x_status b2x_moe_combine_backward(const void* grad, int64_t ld_grad, const void* y, int64_t y_rows,
+                                            int64_t ld_y, const int32_t* rows, const float* weights, int64_t tokens,
+                                            int top_k, int64_t cols, void* d_y, int64_t ld_d_y, float* d_weights,
+                                            b2x_dtype type, void* stream);
+
 /* ------------------------------------------------------------ GEMM + all-reduce */
 
 /*

@@ -28,6 +28,8 @@ EXPORTED = (
     "b2x_read_device_status", "b2x_check_device", "b2x_debug_inject", "b2x_abi_version", "b2x_launch_count", "b2x_fp8_gemm_splitk_noalloc",
     "b2x_trace_read", "b2x_allreduce_signal_words", "b2x_fp8_gemm_allreduce",
     "b2x_stoch_round", "b2x_stoch_round_rs", "b2x_grouped_gemm_workspace_size", "b2x_fp8_grouped_gemm", "b2x_fp8_gemm_swiglu",
+    "b2x_fp8_gemm_epilogue", "b2x_epilogue_backward", "b2x_moe_route", "b2x_moe_route_backward", "b2x_moe_dispatch",
+    "b2x_moe_gemm", "b2x_moe_gemm_swiglu", "b2x_moe_combine", "b2x_moe_combine_backward",
 )
 
 AR_MAX_RANKS = 8
@@ -79,6 +81,49 @@ class GemmGroup(ctypes.Structure):
         ("M", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64),
         ("lda", ctypes.c_int64), ("ldb", ctypes.c_int64), ("ldc", ctypes.c_int64),
         ("scale_a", ctypes.c_void_p), ("scale_b", ctypes.c_void_p),
+    ]
+
+
+class Epilogue(ctypes.Structure):
+    _fields_ = [
+        ("bias", ctypes.c_void_p), ("bias_type", ctypes.c_int), ("activation", ctypes.c_int),
+        ("residual", ctypes.c_void_p), ("ld_residual", ctypes.c_int64),
+        ("pre", ctypes.c_void_p), ("ld_pre", ctypes.c_int64),
+    ]
+
+
+class MoeRouteArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p), ("logits_type", ctypes.c_int),
+        ("tokens", ctypes.c_int64), ("experts", ctypes.c_int64), ("ld_logits", ctypes.c_int64),
+        ("top_k", ctypes.c_int), ("sigmoid", ctypes.c_int), ("bias", ctypes.c_void_p),
+        ("num_groups", ctypes.c_int), ("top_groups", ctypes.c_int), ("group_top2", ctypes.c_int),
+        ("renormalize", ctypes.c_int), ("scale", ctypes.c_float),
+        ("weights", ctypes.c_void_p), ("indices", ctypes.c_void_p),
+    ]
+
+
+class MoeDispatchArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("x_type", ctypes.c_int),
+        ("tokens", ctypes.c_int64), ("cols", ctypes.c_int64), ("ld_x", ctypes.c_int64),
+        ("indices", ctypes.c_void_p), ("top_k", ctypes.c_int), ("experts", ctypes.c_int64),
+        ("q", ctypes.c_void_p), ("q_type", ctypes.c_int), ("ld_q", ctypes.c_int64),
+        ("scale", ctypes.c_void_p), ("given", ctypes.c_void_p),
+        ("offsets", ctypes.c_void_p), ("rows", ctypes.c_void_p),
+    ]
+
+
+class MoeGemmArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("x_type", ctypes.c_int),
+        ("rows", ctypes.c_int64), ("K", ctypes.c_int64), ("ld_x", ctypes.c_int64),
+        ("w", ctypes.c_void_p), ("w_type", ctypes.c_int),
+        ("experts", ctypes.c_int64), ("N", ctypes.c_int64),
+        ("ldw_e", ctypes.c_int64), ("ldw_n", ctypes.c_int64), ("ldw_k", ctypes.c_int64),
+        ("offsets", ctypes.c_void_p),
+        ("scale_x", ctypes.c_void_p), ("scale_x_count", ctypes.c_int64),
+        ("scale_w", ctypes.c_void_p), ("scale_w_count", ctypes.c_int64),
     ]
 
 
@@ -155,6 +200,20 @@ def lib() -> ctypes.CDLL:
                                         ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,
                                         ctypes.c_void_p]
         L.b2x_splitk_reduce.restype = ctypes.c_int
+        vp, i64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
+        for name, args in {
+                "b2x_fp8_gemm_epilogue": [ctypes.POINTER(GemmArgs), ctypes.POINTER(Epilogue), vp],
+                "b2x_epilogue_backward": [vp, i64, vp, i64, vp, i64, vp, i32, i64, i64, i32, vp],
+                "b2x_moe_route": [ctypes.POINTER(MoeRouteArgs), vp],
+                "b2x_moe_route_backward": [ctypes.POINTER(MoeRouteArgs), vp, vp, i64, vp],
+                "b2x_moe_dispatch": [ctypes.POINTER(MoeDispatchArgs), vp],
+                "b2x_moe_gemm": [ctypes.POINTER(MoeGemmArgs), vp, i32, i64, vp],
+                "b2x_moe_gemm_swiglu": [ctypes.POINTER(MoeGemmArgs), vp, i32, i64, vp, vp, vp],
+                "b2x_moe_combine": [vp, i64, i64, vp, vp, i64, i32, i64, vp, i64, vp, i64, i32, vp],
+                "b2x_moe_combine_backward": [vp, i64, vp, i64, i64, vp, vp, i64, i32, i64, vp, i64, vp, i32, vp],
+        }.items():
+            fn = getattr(L, name)
+            fn.argtypes, fn.restype = args, i32
         L.b2x_last_error.argtypes = []
         L.b2x_last_error.restype = ctypes.c_char_p
         L.b2x_check_device.argtypes = []

@@ -1,0 +1,519 @@
+// fp8 products of a feed-forward layer for sm_100a, dense or one per expert over rows sorted by expert, with their
+// epilogues (bias, activation, residual; SwiGLU and fp8).  Weight rows on the tensor core's 128-row side, tokens on its
+// column side; see fp8_gemm_tokens.cuh.  The experts' row ranges are read on the device.
+//
+// fp8_gemm_tokens_kernel: one CTA per 128 weight rows x NT tokens x K range, two CTAs per SM (one's start and end hide
+// behind the other's stream).  The K ranges of a tile are the CTAs of a cluster: each leaves its fp32 partial tile in its
+// own shared memory and the cluster adds them over distributed shared memory in the order of the ranges, so there is no
+// workspace, no atomic, nothing to clear, and the same inputs give the same bits.  For few tokens it is bound by reading
+// the weights once.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include "fp8_gemm_tokens.cuh"
+
+namespace b2x {
+
+constexpr int kTkThreads = 192;  // warps 0-3 read TMEM, warp 4 loads, warp 5 issues the MMAs
+constexpr int kTkWarps = kTkThreads / 32;
+
+template <int NT>
+struct TkSmem {
+  static constexpr int kWBytes = kTkRows * kBK;
+  static constexpr int kXBytes = NT * kBK;
+  static constexpr int kStageBytes = kWBytes + kXBytes;
+  // two CTAs per SM: half of the shared memory each
+  static constexpr int kStages = (kMaxDynSmem / 2 - 2048) / kStageBytes;
+  static constexpr int kXOff = kStages * kWBytes;
+  static constexpr int kBarOff = kStages * kStageBytes;
+  static constexpr int kAlloc = kBarOff + (2 * kStages + 1) * 8 + 16 + 1024;
+  static_assert(kStages * kStageBytes >= NT * kTkRows * 4, "the partial tile reuses the ring");
+};
+
+// Unit `unit` of the grid by one warp: experts in order, weight tiles of an expert, its token tiles innermost (so that
+// the CTAs that share a weight tile run together).
+template <int NT>
+__device__ __forceinline__ TokUnit tok_find_unit(const TokParams& p, int unit, int lane) {
+  TokUnit u{0, 0, 0, 0};
+  if (!p.offsets) {
+    const int mt = (int)((p.rows + NT - 1) / NT);
+    u.nt = unit / mt;
+    if (u.nt >= p.n_tiles) return u;
+    u.row0 = (int64_t)(unit % mt) * NT;
+    u.cnt = (int)min((int64_t)NT, p.rows - u.row0);
+    return u;
+  }
+  int carry = 0;
+  for (int base = 0; base < p.E; base += 32) {
+    int64_t lo = 0, hi = 0;
+    if (base + lane < p.E) tok_range(p, base + lane, lo, hi);
+    const int mt = (int)((hi - lo + NT - 1) / NT);
+    int s = mt * p.n_tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += v;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, unit < carry + s);
+    if (past) {
+      const int src = __ffs(past) - 1;
+      const int local = unit - carry - s + mt * p.n_tiles;  // right on lane src
+      const int m = mt ? local % mt : 0;
+      u.e = base + src;
+      u.nt = __shfl_sync(0xffffffffu, mt ? local / mt : 0, src);
+      u.row0 = __shfl_sync(0xffffffffu, lo + (int64_t)m * NT, src);
+      u.cnt = __shfl_sync(0xffffffffu, (int)min((int64_t)NT, hi - lo - (int64_t)m * NT), src);
+      return u;
+    }
+    carry += __shfl_sync(0xffffffffu, s, 31);
+  }
+  return u;
+}
+
+// The 128 weight rows of tile nt, K block kb.  W_KIND 0: K-major [E][N, K]; 1: row-major [E][K, N]; 2: gate and up rows
+// in turns of 16 (map {K, 16, gate / up, 8, blocks of 256 rows}).
+template <int W_KIND>
+__device__ __forceinline__ void tok_load_w(const TokParams& p, void* dst, const CUtensorMap* m, uint64_t* bar, int kb,
+                                           int e, int nt, uint64_t pol) {
+  if constexpr (W_KIND == 0)
+    tma_load_3d(dst, m, bar, kb * kBK, nt * kTkRows, e, pol);
+  else if constexpr (W_KIND == 1)
+    tma_load_3d(dst, m, bar, nt * kTkRows, kb * kBK, e, pol);
+  else
+    tma_load_5d(dst, m, bar, kb * kBK, 0, 0, (nt & 1) * 4, e * (p.N / 256) + (nt >> 1), pol);
+}
+
+template <int NT, int W_KIND>
+__global__ void __launch_bounds__(kTkThreads, 2)
+    fp8_gemm_tokens_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                           const TokParams p) {
+  using L = TkSmem<NT>;
+  constexpr int S = L::kStages;
+  constexpr uint32_t kTmemCols = NT < 32 ? 32 : NT;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* empty = full + S;
+  uint64_t* done = empty + S;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % p.splits;
+
+  // every warp finds the unit itself: no shared memory, the same result in all CTAs of the cluster
+  const TokUnit u = tok_find_unit<NT>(p, blockIdx.x / p.splits, lane);
+  if (u.cnt == 0) return;  // the whole cluster leaves
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 4 && lane == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+  }
+  if (warp == 5) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int per = (p.k_tiles + p.splits - 1) / p.splits;
+  const int k0 = min(rank * per, p.k_tiles), k1 = min(k0 + per, p.k_tiles);
+
+  if (warp == 4) {
+    if (lane == 0) {
+      const uint64_t pol_w = l2_policy(p.l2_w), pol_x = policy_evict_last();
+      int stage = 0;
+      uint32_t phase = 0, issued = 0, pend[S];
+      for (int kb = k0; kb < k1; ++kb) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, kStatusTimeoutProducer)) break;
+        mbar_arrive_expect_tx(&full[stage], L::kStageBytes);
+        tok_load_w<W_KIND>(p, smem + stage * L::kWBytes, &tmW, &full[stage], kb, u.e, u.nt, pol_w);
+        tma_load_2d(smem + L::kXOff + stage * L::kXBytes, &tmX, &full[stage], kb * kBK, (int)u.row0, pol_x);
+        issued |= 1u << stage;
+        pend[stage] = phase;
+        if (++stage == S) stage = 0, phase ^= 1;
+      }
+      for (int s = 0; s < S; ++s)
+        if (issued & (1u << s)) {
+          volatile int no_abort = 0;
+          mbar_wait(&full[s], pend[s], &no_abort, kStatusTimeoutProducer);
+        }
+    }
+  } else if (warp == 5) {
+    if (lane == 0) {
+      const uint32_t idesc = p.idesc | ((uint32_t)(NT >> 3) << 17);
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = k0; kb < k1; ++kb) {
+        if (!mbar_wait(&full[stage], phase, abort_flag, kStatusTimeoutMma)) break;
+        tc_fence_after();
+        const uint32_t w = smem_u32(smem + stage * L::kWBytes), x = smem_u32(smem + L::kXOff + stage * L::kXBytes);
+#pragma unroll
+        for (int k = 0; k < kBK / 32; ++k)
+          mma_f8f6f4(tmem_base,
+                     W_KIND == 1 ? smem_desc_sw128(w + k * 32 * 128, 128 * kBK, 1024) : smem_desc_sw128(w + k * 32, 16, 1024),
+                     smem_desc_sw128(x + k * 32, 16, 1024), idesc, (kb > k0 || k > 0) ? 1u : 0u);
+        mma_commit(&empty[stage]);
+        if (++stage == S) stage = 0, phase ^= 1;
+      }
+      mma_commit(done);
+      volatile int no_abort = 0;
+      mbar_wait(done, 0, &no_abort, kStatusTimeoutMma);
+    }
+  } else {
+    // the finished partial tile -> shared memory [token][weight row], over the ring that nothing uses any more
+    mbar_wait(done, 0, abort_flag, kStatusTimeoutEpilogue);
+    __syncwarp();
+    tc_fence_after();
+    float* part = reinterpret_cast<float*>(smem) + warp * 32 + lane;
+#pragma unroll
+    for (int c0 = 0; c0 < NT; c0 += 16) {
+      uint32_t v[16];
+      tmem_ld_32x32b_x16(tmem_base + ((uint32_t)(warp * 32) << 16) + c0, v);
+      tmem_ld_wait();
+      tmem_regs_after_wait(v);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) part[(c0 + i) * kTkRows] = k1 > k0 ? __uint_as_float(v[i]) : 0.0f;
+    }
+    tc_fence_before();
+  }
+  __syncwarp();
+  if (p.splits > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  const uint32_t tile = smem_u32(smem);
+  auto fetch = [&](int m, int col) {
+    const uint32_t at = tile + (uint32_t)(m * kTkRows + col) * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p.splits == 1) {
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(s.x), "=f"(s.y), "=f"(s.z), "=f"(s.w) : "r"(at) : "memory");
+    } else {
+      for (int r = 0; r < p.splits; ++r) {
+        float4 f;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
+                     : "r"(mapa_shared(at, r))
+                     : "memory");
+        s.x += f.x, s.y += f.y, s.z += f.z, s.w += f.w;
+      }
+    }
+    return s;
+  };
+  if constexpr (W_KIND == 2) {
+    const float hs = __ldg(p.h_scale);
+    const float inv = hs == 0.0f ? 0.0f : __fdiv_rn(1.0f, hs);
+    float amax = 0.0f;
+    tok_finish_swiglu(p, u.e, u.row0, u.nt * kTkRows, u.cnt, rank * kTkWarps + warp, p.splits * kTkWarps, lane, inv, amax, fetch);
+    if (p.h_amax) {
+      const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
+      if (lane == 0 && m) atomicMax(reinterpret_cast<unsigned*>(p.h_amax), m);
+    }
+  } else {
+    tok_finish(p, u.e, u.row0, u.nt * kTkRows, u.cnt, rank * kTkWarps + warp, p.splits * kTkWarps, lane, fetch);
+  }
+  __syncwarp();
+  if (p.splits > 1)
+    cluster_sync();  // peers may still read this CTA's partial tile
+  else
+    __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+struct TokLaunch {
+  CUtensorMap tmW;
+  TokParams p;
+  const void* x;
+  int64_t ld_x;
+  int w_kind, w_fmt, x_fmt;
+  int num_sms;
+};
+
+template <int NT, int W_KIND>
+static cudaError_t launch_tokens_t(const TokLaunch& g, const CUtensorMap& tmX, int64_t units, cudaStream_t st) {
+  using L = TkSmem<NT>;
+  auto kern = fp8_gemm_tokens_kernel<NT, W_KIND>;
+  cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), L::kAlloc);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * g.p.splits), 1, 1);
+  cfg.blockDim = dim3(kTkThreads, 1, 1);
+  cfg.dynamicSmemBytes = L::kAlloc;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = g.p.splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kern, g.tmW, tmX, g.p);
+  note_launch(1);
+  return e;
+}
+
+template <int NT>
+static cudaError_t launch_tokens_nt(const TokLaunch& g, const CUtensorMap& tmX, int64_t units, cudaStream_t st) {
+  if (g.w_kind == 0) return launch_tokens_t<NT, 0>(g, tmX, units, st);
+  if (g.w_kind == 1) return launch_tokens_t<NT, 1>(g, tmX, units, st);
+  return launch_tokens_t<NT, 2>(g, tmX, units, st);
+}
+
+// Experts that get a row when `rows` fall on E experts evenly: what the grid is planned for.
+static double expected_active(int64_t rows, int64_t E) { return (double)E * (1.0 - pow(1.0 - 1.0 / (double)E, (double)rows)); }
+
+static b2x_status launch_tokens(TokLaunch& g, const char* who, cudaStream_t st) {
+  TokParams& p = g.p;
+  const bool moe = p.offsets != nullptr;
+  const double active = moe ? expected_active(p.rows, p.E) : 1.0;
+  const double mean = (double)p.rows / active;
+  // Token tile: the mean expert fits with room for an uneven spread.
+  int nt = 128;
+  if (mean <= (moe ? 10 : 16)) nt = 16;
+  else if (mean <= (moe ? 20 : 32)) nt = 32;
+  else if (mean <= (moe ? 48 : 64)) nt = 64;
+  // Most units that any spread of the rows can give (sum of ceil(c / nt)); those past the last leave at once.
+  const int64_t tok_tiles = moe ? p.rows / nt + std::min<int64_t>(p.E, p.rows) : (p.rows + nt - 1) / nt;
+  const int64_t units = tok_tiles * p.n_tiles;
+  const double planned = std::max(1.0, moe ? active * ceil(mean / nt) : (double)tok_tiles) * p.n_tiles;
+  // K ranges: as many as fill the SMs' two slots best, a little preference for fewer.
+  double best = -1;
+  for (int s = 1; s <= 8; s *= 2) {
+    const int per = (p.k_tiles + s - 1) / s;
+    if (s > 1 && (per < 4 || (int64_t)(s - 1) * per >= p.k_tiles)) break;
+    const double ctas = planned * s, slots = 2.0 * g.num_sms;
+    const double eff = ctas / (ceil(ctas / slots) * slots) * pow(0.97, log2((double)s));
+    if (eff > best) best = eff, p.splits = s;
+  }
+  if (units * p.splits >= (1LL << 31)) return fail(B2X_ERR_UNSUPPORTED, "%s: too many tiles", who);
+  p.idesc = idesc_f8f6f4(g.w_fmt, g.x_fmt, g.w_kind == 1 ? 1 : 0, 0, kTkRows, 0);
+  p.l2_w = 1;
+  CUtensorMap tmX;
+  b2x_status s = encode_2d(&tmX, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.x, (uint64_t)p.K, (uint64_t)p.rows, (uint64_t)g.ld_x, 128,
+                           (uint32_t)nt, CU_TENSOR_MAP_SWIZZLE_128B, "x");
+  if (s != B2X_OK) return s;
+  cudaError_t e = nt == 16   ? launch_tokens_nt<16>(g, tmX, units, st)
+                  : nt == 32 ? launch_tokens_nt<32>(g, tmX, units, st)
+                  : nt == 64 ? launch_tokens_nt<64>(g, tmX, units, st)
+                             : launch_tokens_nt<128>(g, tmX, units, st);
+  return e == cudaSuccess ? B2X_OK : cuda_fail(e, who);
+}
+
+// Tensor map of the weights, [E][N, K] by strides; see tok_load_w for the kinds.
+static b2x_status encode_weights(CUtensorMap* m, int kind, const void* w, int64_t E, int64_t N, int64_t K, int64_t ld_e,
+                                 int64_t ld) {
+  auto fn = get_encode_fn();
+  if (!fn) return fail(B2X_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint32_t es[5] = {1, 1, 1, 1, 1};
+  CUresult r;
+  if (kind == 2) {
+    cuuint64_t dims[5] = {(cuuint64_t)K, 16, 2, 8, (cuuint64_t)(E * (N / 256))};
+    cuuint64_t strides[4] = {(cuuint64_t)ld, (cuuint64_t)ld * 128, (cuuint64_t)ld * 16, (cuuint64_t)ld * 256};
+    cuuint32_t box[5] = {128, 16, 2, 4, 1};
+    r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(w), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  } else {
+    cuuint64_t dims[3] = {(cuuint64_t)(kind ? N : K), (cuuint64_t)(kind ? K : N), (cuuint64_t)E};
+    cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)(E > 1 ? ld_e : ld * (kind ? K : N))};
+    cuuint32_t box[3] = {128, 128, 1};
+    r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(w), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  }
+  if (r != CUDA_SUCCESS)
+    return fail(B2X_ERR_INVALID_ARG, "cuTensorMapEncodeTiled(weights) failed with %d (experts %lld, N %lld, K %lld)", (int)r,
+                (long long)E, (long long)N, (long long)K);
+  return B2X_OK;
+}
+
+static bool even_rows(const void* p, int64_t ld) { return ((uintptr_t)p % 8) == 0 && ld % 4 == 0; }
+
+static int b2x_device_sms(const char* who, b2x_status& s) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  s = e == cudaSuccess ? B2X_OK : cuda_fail(e, who);
+  return s == B2X_OK ? device_num_sms(dev) : 0;
+}
+
+// Checks and translation shared by b2x_moe_gemm and b2x_moe_gemm_swiglu.
+static b2x_status moe_gemm_params(const b2x_moe_gemm_args* a, const char* who, bool swiglu, TokLaunch& g) {
+  if (!a) return fail(B2X_ERR_INVALID_ARG, "%s: args is NULL", who);
+  if (!is_fp8(a->x_type) || !is_fp8(a->w_type)) return fail(B2X_ERR_UNSUPPORTED, "%s: x and w must be e4m3 or e5m2", who);
+  if (a->rows < 0 || a->K < 0 || a->N < 0 || a->experts < 1)
+    return fail(B2X_ERR_INVALID_ARG, "%s: bad shape (rows %lld, N %lld, K %lld, experts %lld)", who, (long long)a->rows,
+                (long long)a->N, (long long)a->K, (long long)a->experts);
+  if (a->rows >= (1LL << 31) || a->K >= (1LL << 31) || a->N >= (1LL << 31) || a->experts > 1024)
+    return fail(B2X_ERR_UNSUPPORTED, "%s: dimensions must be < 2^31, experts at most 1024", who);
+  if (a->rows == 0 || a->N == 0) return B2X_OK;
+  if (a->K == 0) return fail(B2X_ERR_UNSUPPORTED, "%s: K == 0", who);
+  if (!a->x || !a->w || !a->offsets) return fail(B2X_ERR_INVALID_ARG, "%s: NULL x, w or offsets", who);
+  if (a->ld_x < a->K || a->ld_x % 16 || (uintptr_t)a->x % 16)
+    return fail(B2X_ERR_INVALID_ARG, "%s: x must be 16-byte aligned with ld_x >= K and ld_x %% 16 == 0", who);
+  int64_t ld;
+  if (a->ldw_k == 1 && a->ldw_n >= a->K) {
+    g.w_kind = 0;
+    ld = a->ldw_n;
+  } else if (a->ldw_n == 1 && a->ldw_k >= a->N) {
+    g.w_kind = 1;
+    ld = a->ldw_k;
+  } else {
+    return fail(B2X_ERR_INVALID_ARG, "%s: w strides (%lld, %lld) are not K-major or row-major", who, (long long)a->ldw_n,
+                (long long)a->ldw_k);
+  }
+  if (ld % 16 || (uintptr_t)a->w % 16 || (a->experts > 1 && (a->ldw_e % 16 || a->ldw_e < 0)))
+    return fail(B2X_ERR_INVALID_ARG, "%s: w must be 16-byte aligned with strides that are multiples of 16", who);
+  if ((a->scale_x && a->scale_x_count != 1 && a->scale_x_count != a->rows) ||
+      (a->scale_w && a->scale_w_count != 1 && a->scale_w_count != a->experts))
+    return fail(B2X_ERR_INVALID_ARG, "%s: scale_x has one element or one per row, scale_w one or one per expert", who);
+  if (swiglu) {
+    if (g.w_kind != 0) return fail(B2X_ERR_UNSUPPORTED, "%s: w must be K-major", who);
+    if (a->N % 256) return fail(B2X_ERR_UNSUPPORTED, "%s: N (gate + up rows) must be a multiple of 256", who);
+    if (a->experts > 1 && a->ldw_e != a->N * ld)
+      return fail(B2X_ERR_UNSUPPORTED, "%s: the experts' weights must lie one after the other (ldw_e = N * ldw_n)", who);
+    g.w_kind = 2;
+  }
+  b2x_status s;
+  g.num_sms = b2x_device_sms(who, s);
+  if (s != B2X_OK) return s;
+  s = encode_weights(&g.tmW, g.w_kind, a->w, a->experts, a->N, a->K, a->ldw_e, ld);
+  if (s != B2X_OK) return s;
+  g.x = a->x;
+  g.ld_x = a->ld_x;
+  g.w_fmt = a->w_type == B2X_E4M3 ? 0 : 1;
+  g.x_fmt = a->x_type == B2X_E4M3 ? 0 : 1;
+  TokParams& p = g.p;
+  p.N = (int)a->N;
+  p.K = (int)a->K;
+  p.E = (int)a->experts;
+  p.rows = a->rows;
+  p.offsets = a->offsets;
+  p.n_tiles = (int)((a->N + kTkRows - 1) / kTkRows);
+  p.k_tiles = (int)((a->K + kBK - 1) / kBK);
+  p.scale_x = a->scale_x;
+  p.scale_w = a->scale_w;
+  p.sx_mode = !a->scale_x ? 0 : (a->scale_x_count == 1 && a->rows != 1 ? 1 : 2);
+  p.sw_mode = !a->scale_w ? 0 : (a->scale_w_count == 1 ? 1 : 2);
+  return B2X_OK;
+}
+
+}  // namespace b2x
+
+extern "C" B2X_API b2x_status b2x_moe_gemm(const b2x_moe_gemm_args* a, void* y, b2x_dtype y_type, int64_t ld_y, void* stream) {
+  using namespace b2x;
+  t_err[0] = 0;
+  if (y_type != B2X_BF16 && y_type != B2X_F16) return fail(B2X_ERR_UNSUPPORTED, "b2x_moe_gemm: y must be bf16 or fp16");
+  TokLaunch g{};
+  b2x_status s = moe_gemm_params(a, "b2x_moe_gemm", false, g);
+  if (s != B2X_OK || a->rows == 0 || a->N == 0) return s;
+  if (!y || ld_y < a->N || (uintptr_t)y % 2) return fail(B2X_ERR_INVALID_ARG, "b2x_moe_gemm: NULL y or ld_y < N");
+  g.p.out = reinterpret_cast<uint16_t*>(y);
+  g.p.ld_out = ld_y;
+  g.p.half = y_type == B2X_F16;
+  g.p.vec_out = even_rows(y, ld_y);
+  return launch_tokens(g, "b2x_moe_gemm launch", (cudaStream_t)stream);
+}
+
+extern "C" B2X_API b2x_status b2x_moe_gemm_swiglu(const b2x_moe_gemm_args* a, void* h, b2x_dtype h_type, int64_t ld_h,
+                                                  const float* h_scale, float* h_amax, void* stream) {
+  using namespace b2x;
+  t_err[0] = 0;
+  if (!is_fp8(h_type)) return fail(B2X_ERR_UNSUPPORTED, "b2x_moe_gemm_swiglu: h must be e4m3 or e5m2");
+  TokLaunch g{};
+  b2x_status s = moe_gemm_params(a, "b2x_moe_gemm_swiglu", true, g);
+  if (s != B2X_OK || a->rows == 0 || a->N == 0) return s;
+  if (!h || ld_h < a->N / 2 || ld_h % 16 || (uintptr_t)h % 16)
+    return fail(B2X_ERR_INVALID_ARG, "b2x_moe_gemm_swiglu: h must be 16-byte aligned with ld_h >= N/2 and ld_h %% 16 == 0");
+  if (!h_scale) return fail(B2X_ERR_INVALID_ARG, "b2x_moe_gemm_swiglu: NULL h_scale");
+  g.p.h = reinterpret_cast<uint8_t*>(h);
+  g.p.ld_h = ld_h;
+  g.p.h_e5m2 = h_type == B2X_E5M2;
+  g.p.h_scale = h_scale;
+  g.p.h_amax = h_amax;
+  return launch_tokens(g, "b2x_moe_gemm_swiglu launch", (cudaStream_t)stream);
+}
+
+extern "C" B2X_API b2x_status b2x_fp8_gemm_epilogue(const b2x_gemm_args* a, const b2x_epilogue* ep, void* stream) {
+  using namespace b2x;
+  t_err[0] = 0;
+  if (!a || !ep) return fail(B2X_ERR_INVALID_ARG, "b2x_fp8_gemm_epilogue: NULL argument");
+  if (!is_fp8(a->a_type) || !is_fp8(a->b_type)) return fail(B2X_ERR_UNSUPPORTED, "b2x_fp8_gemm_epilogue: A and B must be e4m3 or e5m2");
+  if (a->c_type != B2X_BF16 && a->c_type != B2X_F16) return fail(B2X_ERR_UNSUPPORTED, "b2x_fp8_gemm_epilogue: C must be bf16 or fp16");
+  if (a->M < 0 || a->N < 0 || a->K < 0) return fail(B2X_ERR_INVALID_ARG, "b2x_fp8_gemm_epilogue: negative shape");
+  if (a->M >= (1LL << 31) || a->N >= (1LL << 31) || a->K >= (1LL << 31))
+    return fail(B2X_ERR_UNSUPPORTED, "b2x_fp8_gemm_epilogue: dimensions must be < 2^31");
+  if (!valid_activation(ep->activation))
+    return fail(B2X_ERR_INVALID_ARG, "b2x_fp8_gemm_epilogue: unknown activation %d", (int)ep->activation);
+  if (ep->bias && !is_float_type(ep->bias_type))
+    return fail(B2X_ERR_UNSUPPORTED, "b2x_fp8_gemm_epilogue: bias must be fp32, bf16 or fp16");
+  if (a->scale_mode != B2X_SCALE_NONE && a->scale_mode != B2X_SCALE_TENSOR && a->scale_mode != B2X_SCALE_TENSOR_GIVEN)
+    return fail(B2X_ERR_UNSUPPORTED, "b2x_fp8_gemm_epilogue: takes per-tensor scales or none");
+  if (a->M == 0 || a->N == 0) return B2X_OK;
+  if (a->K == 0) return fail(B2X_ERR_UNSUPPORTED, "b2x_fp8_gemm_epilogue: K == 0");
+  if (!a->a || !a->b || !a->c) return fail(B2X_ERR_INVALID_ARG, "b2x_fp8_gemm_epilogue: NULL A, B or C");
+  if (a->scale_mode != B2X_SCALE_NONE && (!a->scale_a || !a->scale_b))
+    return fail(B2X_ERR_INVALID_ARG, "b2x_fp8_gemm_epilogue: NULL scale pointer");
+  if (a->lda < a->K || a->lda % 16 || (uintptr_t)a->a % 16)
+    return fail(B2X_ERR_INVALID_ARG, "b2x_fp8_gemm_epilogue: A must be 16-byte aligned with lda >= K and lda %% 16 == 0");
+  TokLaunch g{};
+  int64_t ld;
+  if (a->ldb_k == 1 && a->ldb_n >= a->K) {
+    g.w_kind = 0;
+    ld = a->ldb_n;
+  } else if (a->ldb_n == 1 && a->ldb_k >= a->N) {
+    g.w_kind = 1;
+    ld = a->ldb_k;
+  } else {
+    return fail(B2X_ERR_INVALID_ARG, "b2x_fp8_gemm_epilogue: B strides (%lld, %lld) are not K-major or row-major",
+                (long long)a->ldb_k, (long long)a->ldb_n);
+  }
+  if (ld % 16 || (uintptr_t)a->b % 16)
+    return fail(B2X_ERR_INVALID_ARG, "b2x_fp8_gemm_epilogue: B needs 16-byte alignment and a row stride %% 16 == 0");
+  if (a->ldc < a->N || (uintptr_t)a->c % 2 || (ep->residual && ep->ld_residual < a->N) || (ep->pre && ep->ld_pre < a->N))
+    return fail(B2X_ERR_INVALID_ARG, "b2x_fp8_gemm_epilogue: row strides of C, residual and pre must be >= N");
+  b2x_status s;
+  g.num_sms = b2x_device_sms("b2x_fp8_gemm_epilogue", s);
+  if (s != B2X_OK) return s;
+  s = encode_weights(&g.tmW, g.w_kind, a->b, 1, a->N, a->K, 0, ld);
+  if (s != B2X_OK) return s;
+  g.x = a->a;
+  g.ld_x = a->lda;
+  g.w_fmt = a->b_type == B2X_E4M3 ? 0 : 1;
+  g.x_fmt = a->a_type == B2X_E4M3 ? 0 : 1;
+  TokParams& p = g.p;
+  p.N = (int)a->N;
+  p.K = (int)a->K;
+  p.E = 1;
+  p.rows = a->M;
+  p.n_tiles = (int)((a->N + kTkRows - 1) / kTkRows);
+  p.k_tiles = (int)((a->K + kBK - 1) / kBK);
+  if (a->scale_mode != B2X_SCALE_NONE) {
+    p.scale_x = a->scale_a;
+    p.scale_w = a->scale_b;
+    p.sx_mode = p.sw_mode = 1;
+  }
+  p.half = a->c_type == B2X_F16;
+  p.bias = ep->bias;
+  p.bias_type = ep->bias_type;
+  p.act = ep->activation;
+  p.residual = reinterpret_cast<const uint16_t*>(ep->residual);
+  p.ld_res = ep->ld_residual;
+  p.vec_res = even_rows(ep->residual, ep->ld_residual);
+  p.out = reinterpret_cast<uint16_t*>(a->c);
+  p.ld_out = a->ldc;
+  p.vec_out = even_rows(a->c, a->ldc);
+  p.pre = reinterpret_cast<uint16_t*>(ep->pre);
+  p.ld_pre = ep->ld_pre;
+  p.vec_pre = even_rows(ep->pre, ep->ld_pre);
+  return launch_tokens(g, "b2x_fp8_gemm_epilogue launch", (cudaStream_t)stream);
+}

@@ -1,0 +1,500 @@
+// Expert routing for sm_100a: scores, balance bias, groups, top-k and renormalised weights of a mixture of experts, and
+// the gradient of the weights.
+//
+// One warp owns a token; lane l holds the logits of experts 32 i + l in registers, so a row is read once, coalesced.
+// The k choices are taken one after the other: a warp-wide maximum of order-preserving 32-bit keys (redux.sync), then the
+// lowest index that has it.
+//
+// What is compared.  Without a bias s is monotone in the logit, so the logits themselves are the keys and the choice is
+// exact.  With a bias (and for sums of two) the keys are fp32 values of s + b, each off by at most
+// `err` = (2^-20 + softmax: (VPL + 5) 2^-24) max s + 2^-23 max |s + b|: the fast exponential and division together stay
+// below 2^-20 relative, the softmax's sum adds VPL + 5 roundings, and s + b is rounded once.  A row whose chosen values
+// lie closer than 2 err, or whose group scores (sums of two, 3 err each) lie closer than 6 err at the border, is chosen
+// again in fp64 (choose_exact): the choice is right to fp64, at the speed of fp32 for nearly all rows.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cstdint>
+#include "activations.cuh"
+#include "b2x_internal.h"
+#include "b2x_ptx.cuh"
+
+namespace b2x {
+
+constexpr int kRouteWarps = 4;  // tokens per CTA
+constexpr uint32_t kAll = 0xffffffffu;
+
+struct RouteParams {
+  const void* logits;
+  int64_t ld;
+  int64_t tokens;
+  int type, E, k;
+  int sigmoid, renorm, groups, top_groups, top2;
+  float scale;
+  const float* bias;
+  float* weights;
+  int32_t* indices;
+  // backward
+  const float* d_weights;
+  void* d_logits;
+  int64_t ld_d;
+};
+
+// Unsigned order of floats: masked (-inf) 0, then rising, NaN on top; -0 and +0 are one value.
+__device__ __forceinline__ uint32_t order_key(float f) {
+  if (f != f) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(f + 0.0f);
+  return u == 0xff800000u ? 0u : (u & 0x80000000u ? ~u : u | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {  // of a key that is neither masked nor NaN
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {  // of numbers; NaN is ignored
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
+  return v;
+}
+
+// The largest (value, lowest index) pair of the warp, in fp64; index INT_MAX: none.
+__device__ __forceinline__ void warp_argmax(double& v, int& at) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const double v2 = __shfl_xor_sync(kAll, v, o);
+    const int a2 = __shfl_xor_sync(kAll, at, o);
+    if (v2 > v || (v2 == v && a2 < at)) v = v2, at = a2;
+  }
+}
+
+// The choice in fp64 (rows with values next to a border): lane j < k gets its expert or -1.
+template <int VPL>
+__device__ __noinline__ int choose_exact(const RouteParams& p, const float (&l)[VPL], int lane) {
+  double c[VPL], s[VPL];
+  bool off[VPL];
+  double m = -INFINITY, sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) m = fmax(m, (double)l[i]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmax(m, __shfl_xor_sync(kAll, m, o));
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    s[i] = p.sigmoid ? 1.0 / (1.0 + exp(-(double)l[i])) : exp((double)l[i] - m);
+    if (l[i] == -INFINITY) s[i] = 0.0;
+    sum += s[i];
+  }
+  sum = warp_sum(sum);
+  const int gs = p.E / p.groups;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const int e = 32 * i + lane;
+    if (!p.sigmoid) s[i] /= sum;
+    const float b = p.bias && e < p.E ? p.bias[e] : 0.0f;
+    c[i] = p.bias ? s[i] + (double)b : (double)l[i];
+    s[i] += (double)b;  // what groups are scored by
+    off[i] = e >= p.E || l[i] == -INFINITY || b == -INFINITY;
+    if (c[i] != c[i]) c[i] = INFINITY;
+    if (s[i] != s[i]) s[i] = INFINITY;
+  }
+  if (p.groups > 1) {
+    // every lane keeps the scores of groups lane, lane + 32, ... (groups <= experts <= 1024)
+    bool kept_here[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) kept_here[i] = false;
+    double gv[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) gv[i] = -INFINITY;
+    for (int g = 0; g < p.groups; ++g) {
+      double total = 0.0;
+      bool any = false;
+      int skip = -1;
+      for (int round = 0; round < (p.top2 ? 2 : 1); ++round) {
+        double v = -INFINITY;
+        int at = 0x7fffffff;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+          const int e = 32 * i + lane;
+          if (!off[i] && e / gs == g && e != skip && (s[i] > v || at == 0x7fffffff)) v = s[i], at = e;
+        }
+        warp_argmax(v, at);
+        if (at != 0x7fffffff) total += v, any = true, skip = at;
+      }
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (32 * i + lane == g && any) gv[i] = total;
+    }
+    for (int n = 0; n < p.top_groups; ++n) {
+      double v = -INFINITY;
+      int at = 0x7fffffff;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (32 * i + lane < p.groups && gv[i] > v) v = gv[i], at = 32 * i + lane;
+      warp_argmax(v, at);
+      if (at == 0x7fffffff) break;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        if (32 * i + lane == at) gv[i] = -INFINITY;
+        if ((32 * i + lane) / gs == at) kept_here[i] = true;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) off[i] = off[i] || !kept_here[i];
+  }
+  int mine = -1;
+  for (int j = 0; j < p.k; ++j) {
+    double v = -INFINITY;
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (!off[i] && (c[i] > v || at == 0x7fffffff)) v = c[i], at = 32 * i + lane;
+    warp_argmax(v, at);
+    if (at == 0x7fffffff) break;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (32 * i + lane == at) off[i] = true;
+    if (lane == j) mine = at;
+  }
+  return mine;
+}
+
+// Largest key of the warp and the lowest expert that has it.
+template <int VPL>
+__device__ __forceinline__ uint32_t take_max(const uint32_t (&key)[VPL], int lane, int& at) {
+  uint32_t best = 0;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) best = max(best, key[i]);
+  best = __reduce_max_sync(kAll, best);
+  uint32_t e = 0xffffffffu;
+#pragma unroll
+  for (int i = VPL - 1; i >= 0; --i)
+    if (key[i] == best) e = 32 * i + lane;
+  at = (int)__reduce_min_sync(kAll, e);
+  return best;
+}
+
+template <int VPL>
+__global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(const RouteParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
+  if (t >= p.tokens) return;
+  const int64_t row = t * p.ld;
+  float l[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) l[i] = 32 * i + lane < p.E ? load_f32(p.logits, row + 32 * i + lane, p.type) : -INFINITY;
+
+  float m = -INFINITY, sum = 1.0f;
+  const bool values = p.bias || (p.groups > 1 && p.top2);  // choices or group scores are sums of rounded numbers
+  const bool need_sum = !p.sigmoid && (values || !p.renorm);
+  if (need_sum) {
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) m = fmaxf(m, l[i]), nan |= l[i] != l[i];
+    m = warp_max(m);
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) sum += l[i] == -INFINITY ? 0.0f : __expf(l[i] - m);
+    sum = warp_sum(sum);
+    if (__any_sync(kAll, nan)) sum = NAN;
+  }
+  uint32_t key[VPL];
+  float sc[VPL];  // s + b where `values`
+  float err = 0.0f;
+  if (values) {
+    float hi_s = 0.0f, hi_c = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int e = 32 * i + lane;
+      const float s = l[i] == -INFINITY ? 0.0f : (p.sigmoid ? sigma_fast(l[i]) : __fdividef(__expf(l[i] - m), sum));
+      const float b = p.bias && e < p.E ? __ldg(p.bias + e) : 0.0f;
+      sc[i] = l[i] == -INFINITY || b == -INFINITY ? -INFINITY : s + b;
+      hi_s = fmaxf(hi_s, s);
+      if (fabsf(sc[i]) < INFINITY) hi_c = fmaxf(hi_c, fabsf(sc[i]));
+      key[i] = order_key(p.bias ? sc[i] : l[i]);
+    }
+    err = (0x1p-20f + (p.sigmoid ? 0.0f : (VPL + 5) * 0x1p-24f)) * warp_max(hi_s) + 0x1p-23f * warp_max(hi_c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) key[i] = order_key(l[i]);
+  }
+  bool close = false;  // something to be told apart in fp64
+  if (p.groups > 1) {
+    const int gs = p.E / p.groups;
+    uint32_t gk[VPL];  // lane l: groups l, l + 32, ...
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) gk[i] = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      uint32_t a = 0, b = 0;  // the lane's two largest of the group
+      const int lo = g * gs - lane, hi = lo + gs;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        const uint32_t v = 32 * i >= lo && 32 * i < hi ? (p.top2 ? order_key(sc[i]) : key[i]) : 0u;
+        b = max(b, min(a, v));
+        a = max(a, v);
+      }
+      uint32_t score = __reduce_max_sync(kAll, a);
+      if (p.top2) {
+        const uint32_t who = __ballot_sync(kAll, a == score);
+        const uint32_t second = __reduce_max_sync(kAll, lane == __ffs(who) - 1 ? b : a);
+        if (second != 0 && score != 0xffffffffu) score = order_key(key_value(score) + (second == 0xffffffffu ? NAN : key_value(second)));
+      }
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (32 * i + lane == g) gk[i] = score;
+    }
+    bool kept[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) kept[i] = false;
+    uint32_t last = 0;
+    for (int n = 0; n < p.top_groups; ++n) {
+      int at;
+      const uint32_t best = take_max<VPL>(gk, lane, at);
+      if (best == 0) break;
+      last = best;
+      const int lo = at * gs - lane, hi = lo + gs;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        if (32 * i + lane == at) gk[i] = 0;
+        if (32 * i >= lo && 32 * i < hi) kept[i] = true;
+      }
+    }
+    if (values && last != 0) {  // the border between the groups that stay and those that go
+      int at;
+      const uint32_t next = take_max<VPL>(gk, lane, at);
+      if (next != 0 && last != 0xffffffffu && next != 0xffffffffu) close = !(key_value(last) - key_value(next) > 6.0f * err);
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (!kept[i]) key[i] = 0;
+  }
+  int mine = -1;
+  uint32_t before = 0;
+  int before_at = 0;
+  for (int j = 0; j < p.k + (p.bias ? 1 : 0); ++j) {
+    int at;
+    const uint32_t best = take_max<VPL>(key, lane, at);
+    if (best == 0) break;
+    if (p.bias && j > 0 && before != 0xffffffffu) {
+      // equal logits with equal biases are a true tie, which the index decides
+      const bool near = !(key_value(before) - key_value(best) > 2.0f * err);
+      if (near) {
+        const float la = load_f32(p.logits, row + before_at, p.type), lb = load_f32(p.logits, row + at, p.type);
+        if (!(la == lb && __ldg(p.bias + before_at) == __ldg(p.bias + at))) close = true;
+      }
+    }
+    before = best;
+    before_at = at;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (32 * i + lane == at) key[i] = 0;
+    if (lane == j && j < p.k) mine = at;
+  }
+  if (close) mine = choose_exact<VPL>(p, l, lane);  // uniform over the warp
+
+  // lane j: the weight of its expert
+  float w = 0.0f;
+  const float lm = mine >= 0 ? load_f32(p.logits, row + mine, p.type) : -INFINITY;
+  if (p.sigmoid) {
+    if (mine >= 0) w = sigma_fast(lm);
+    if (p.renorm) {
+      const float total = warp_sum(w);
+      w = total == 0.0f ? 0.0f : __fdiv_rn(w, total);
+    }
+  } else if (p.renorm) {  // softmax over the chosen ones: the common factor cancels
+    const float top = warp_max(lm);
+    if (mine >= 0) w = __expf(lm - top);
+    const float total = warp_sum(w);
+    w = mine >= 0 ? __fdiv_rn(w, total) : 0.0f;
+  } else if (mine >= 0) {
+    w = __fdiv_rn(__expf(lm - m), sum);
+  }
+  if (lane < p.k) {
+    p.weights[t * p.k + lane] = mine >= 0 ? w * p.scale : 0.0f;
+    p.indices[t * p.k + lane] = mine;
+  }
+}
+
+__device__ __forceinline__ void store_f32(void* p, int64_t i, int type, float v) {
+  if (type == B2X_F32)
+    reinterpret_cast<float*>(p)[i] = v;
+  else if (type == B2X_BF16)
+    reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else
+    reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// d_logits of one token per warp.  With w_j = scale s_j (/ S, S = sum of the chosen s):
+//   ds_j = scale d_j                              or  scale (d_j - sum_i d_i s_i / S) / S
+//   sigmoid:  dl_e = ds_e s_e (1 - s_e)
+//   softmax:  dl_e = s_e (ds_e - sum_i s_i ds_i); renormalised, w / scale is the softmax p over the chosen ones and
+//             dl_e = scale p_e (d_e - sum_i p_i d_i), which needs the chosen logits alone.
+// An expert named in two slots gets the sum of both.  The rest of the row is the dense part (0 except for the
+// softmax over all experts), stored first; the chosen ones are stored over it after a __syncwarp.
+template <int VPL>
+__global__ void __launch_bounds__(kRouteWarps * 32) moe_route_backward_kernel(const RouteParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
+  if (t >= p.tokens) return;
+  const int64_t row = t * p.ld;
+  int at = -1;
+  float d = 0.0f, lm = -INFINITY;
+  if (lane < p.k) {
+    at = p.indices[t * p.k + lane];
+    if (at < 0 || at >= p.E) at = -1;
+    if (at >= 0) d = p.d_weights[t * p.k + lane] * p.scale, lm = load_f32(p.logits, row + at, p.type);
+    if (lm == -INFINITY) at = -1, d = 0.0f;
+  }
+  const bool dense = !p.sigmoid && !p.renorm;
+  float mine = 0.0f;
+  if (dense) {
+    float l[VPL];
+    float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      l[i] = 32 * i + lane < p.E ? load_f32(p.logits, row + 32 * i + lane, p.type) : -INFINITY;
+      m = fmaxf(m, l[i]);
+    }
+    m = warp_max(m);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      l[i] = l[i] == -INFINITY ? 0.0f : __expf(l[i] - m);
+      sum += l[i];
+    }
+    sum = warp_sum(sum);
+    const float r = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+    const float s = at >= 0 ? __expf(lm - m) * r : 0.0f;
+    const float mean = warp_sum(at >= 0 ? s * d : 0.0f);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (32 * i + lane < p.E) store_f32(p.d_logits, t * p.ld_d + 32 * i + lane, p.type, -l[i] * r * mean);
+    float all = 0.0f;  // of every slot that names this lane's expert
+    for (int j = 0; j < p.k; ++j) {
+      const int aj = __shfl_sync(kAll, at, j);
+      const float dj = __shfl_sync(kAll, d, j);
+      if (aj == at) all += dj;
+    }
+    mine = s * (all - mean);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (32 * i + lane < p.E) store_f32(p.d_logits, t * p.ld_d + 32 * i + lane, p.type, 0.0f);
+    float dl = 0.0f;  // this slot's part
+    if (p.sigmoid) {
+      const float s = at >= 0 ? sigma_fast(lm) : 0.0f;
+      const float slope = at >= 0 ? s * sigma_fast(-lm) : 0.0f;
+      if (p.renorm) {
+        const float total = warp_sum(s);
+        const float mean = total == 0.0f ? 0.0f : __fdiv_rn(warp_sum(d * s), total);
+        dl = total == 0.0f ? 0.0f : __fdiv_rn((d - mean) * slope, total);
+      } else {
+        dl = d * slope;
+      }
+    } else {
+      const float top = warp_max(lm);
+      float pr = at >= 0 ? __expf(lm - top) : 0.0f;
+      const float total = warp_sum(pr);
+      pr = at >= 0 ? __fdiv_rn(pr, total) : 0.0f;
+      const float mean = warp_sum(at >= 0 ? pr * d : 0.0f);
+      dl = at >= 0 ? pr * (d - mean) : 0.0f;
+    }
+    for (int j = 0; j < p.k; ++j) {
+      const int aj = __shfl_sync(kAll, at, j);
+      const float dj = __shfl_sync(kAll, dl, j);
+      if (aj == at) mine += dj;
+    }
+  }
+  __syncwarp();
+  if (at >= 0) store_f32(p.d_logits, t * p.ld_d + at, p.type, mine);
+}
+
+template <int BACKWARD>
+static cudaError_t launch_route(const RouteParams& p, cudaStream_t st) {
+  const unsigned grid = (unsigned)((p.tokens + kRouteWarps - 1) / kRouteWarps);
+  const int per = (p.E + 31) / 32;
+#define B2X_ROUTE(V)                                                       \
+  if constexpr (BACKWARD)                                                  \
+    moe_route_backward_kernel<V><<<grid, kRouteWarps * 32, 0, st>>>(p);    \
+  else                                                                     \
+    moe_route_kernel<V><<<grid, kRouteWarps * 32, 0, st>>>(p)
+  if (per <= 1) { B2X_ROUTE(1); }
+  else if (per <= 2) { B2X_ROUTE(2); }
+  else if (per <= 4) { B2X_ROUTE(4); }
+  else if (per <= 8) { B2X_ROUTE(8); }
+  else if (per <= 16) { B2X_ROUTE(16); }
+  else { B2X_ROUTE(32); }
+#undef B2X_ROUTE
+  note_launch(1);
+  return cudaGetLastError();
+}
+
+static b2x_status route_params(const b2x_moe_route_args* a, const char* who, bool backward, RouteParams& p) {
+  if (!a) return fail(B2X_ERR_INVALID_ARG, "%s: args is NULL", who);
+  if (a->logits_type != B2X_F32 && a->logits_type != B2X_BF16 && a->logits_type != B2X_F16)
+    return fail(B2X_ERR_UNSUPPORTED, "%s: logits must be fp32, bf16 or fp16", who);
+  if (a->tokens < 0 || a->experts <= 0 || a->ld_logits < a->experts)
+    return fail(B2X_ERR_INVALID_ARG, "%s: bad shape (tokens %lld, experts %lld, ld %lld)", who, (long long)a->tokens,
+                (long long)a->experts, (long long)a->ld_logits);
+  if (a->experts > 1024 || a->top_k > 32)
+    return fail(B2X_ERR_UNSUPPORTED, "%s: at most 1024 experts and top_k 32 (got %lld, %d)", who, (long long)a->experts,
+                a->top_k);
+  if (a->top_k < 1 || a->top_k > a->experts)
+    return fail(B2X_ERR_INVALID_ARG, "%s: top_k must be in [1, experts] (got %d)", who, a->top_k);
+  if (a->tokens > (int64_t)kRouteWarps * 0x7fffffff) return fail(B2X_ERR_UNSUPPORTED, "%s: too many tokens", who);
+  if (!backward && (a->num_groups < 1 || a->experts % a->num_groups || a->top_groups < 1 || a->top_groups > a->num_groups))
+    return fail(B2X_ERR_INVALID_ARG, "%s: num_groups (%d) must divide experts, top_groups (%d) lie in [1, num_groups]", who,
+                a->num_groups, a->top_groups);
+  if (a->tokens > 0 && (!a->logits || !a->indices || (!backward && !a->weights)))
+    return fail(B2X_ERR_INVALID_ARG, "%s: NULL pointer", who);
+  p.logits = a->logits;
+  p.ld = a->ld_logits;
+  p.tokens = a->tokens;
+  p.type = a->logits_type;
+  p.E = (int)a->experts;
+  p.k = a->top_k;
+  p.sigmoid = a->sigmoid != 0;
+  p.renorm = a->renormalize != 0;
+  p.groups = backward || a->top_groups == a->num_groups ? 1 : a->num_groups;  // all groups stay: no group step
+  p.top_groups = a->top_groups;
+  p.top2 = a->group_top2 != 0;
+  p.scale = a->scale;
+  p.bias = a->bias;
+  p.weights = a->weights;
+  p.indices = a->indices;
+  return B2X_OK;
+}
+
+}  // namespace b2x
+
+extern "C" B2X_API b2x_status b2x_moe_route(const b2x_moe_route_args* args, void* stream) {
+  using namespace b2x;
+  t_err[0] = 0;
+  RouteParams p{};
+  b2x_status s = route_params(args, "b2x_moe_route", false, p);
+  if (s != B2X_OK || p.tokens == 0) return s;
+  cudaError_t e = launch_route<0>(p, (cudaStream_t)stream);
+  return e == cudaSuccess ? B2X_OK : cuda_fail(e, "b2x_moe_route launch");
+}
+
+extern "C" B2X_API b2x_status b2x_moe_route_backward(const b2x_moe_route_args* args, const float* d_weights, void* d_logits,
+                                                     int64_t ld_d_logits, void* stream) {
+  using namespace b2x;
+  t_err[0] = 0;
+  RouteParams p{};
+  b2x_status s = route_params(args, "b2x_moe_route_backward", true, p);
+  if (s != B2X_OK) return s;
+  if (ld_d_logits < p.E) return fail(B2X_ERR_INVALID_ARG, "b2x_moe_route_backward: ld_d_logits < experts");
+  if (p.tokens == 0) return B2X_OK;
+  if (!d_weights || !d_logits) return fail(B2X_ERR_INVALID_ARG, "b2x_moe_route_backward: NULL pointer");
+  p.d_weights = d_weights;
+  p.d_logits = d_logits;
+  p.ld_d = ld_d_logits;
+  cudaError_t e = launch_route<1>(p, (cudaStream_t)stream);
+  return e == cudaSuccess ? B2X_OK : cuda_fail(e, "b2x_moe_route_backward launch");
+}

@@ -1,0 +1,606 @@
+// Dispatch and combine of a mixture of experts for sm_100a.
+//
+// Dispatch sorts the (token, slot) pairs stably by expert and writes each token's row, quantized to fp8 once, to all of
+// its places.  The sort is a counting sort:
+//   * up to kFusedPairs pairs, every CTA of the row kernel counts all pairs itself (they are a few KB) and ranks its own
+//     token's: one launch;
+//   * above, one cluster of 8 CTAs (moe_plan_kernel) counts and ranks contiguous eighths of the pairs, its warps
+//     contiguous parts of those; counts meet in shared memory, the CTAs' over distributed shared memory.  No global
+//     counters, no atomics whose order matters: the same input gives the same order.
+// Row kernel: one CTA per token reads the row once (it stays in registers between the maximum and the cast) and stores
+// top_k copies, 16 bytes a thread.  Bound: HBM, tokens * cols * (4 or 2) bytes in and tokens * top_k * cols out.
+//
+// Combine reads the top_k rows of a token side by side (top_k 16-byte loads in flight per thread) and adds them in the
+// order of the slots in fp32.  Bound: HBM.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cstdint>
+#include "activations.cuh"
+#include "b2x_internal.h"
+#include "b2x_ptx.cuh"
+
+namespace b2x {
+
+constexpr int kRowThreads = 128;
+constexpr int kFusedPairs = 2048;   // pairs that a CTA counts by itself
+constexpr int kPlanCtas = 8;
+constexpr int kPlanThreads = 512;
+constexpr int kPlanWarps = kPlanThreads / 32;
+
+struct DispatchParams {
+  const void* x;
+  int x_f32;
+  int64_t tokens, cols, ld_x;
+  const int32_t* indices;
+  int k, E;
+  uint8_t* q;
+  int q_e5m2;
+  int64_t ld_q;
+  float* scale;
+  const float* given;
+  int32_t* offsets;
+  int32_t* rows;
+  int fused;  // ranks are computed here, not read from rows
+  int vec;    // x rows are 16-byte aligned, q rows too
+};
+
+// Exclusive sums of cnt[0..E) in place by the whole CTA; cnt[E] receives the total.
+__device__ __forceinline__ void block_exclusive_scan(int* cnt, int E, int* warp_part) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  int carry = 0;
+  for (int base = 0; base < E; base += blockDim.x) {
+    const int i = base + threadIdx.x;
+    const int v = i < E ? cnt[i] : 0;
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    if (lane == 31) warp_part[warp] = s;
+    __syncthreads();
+    int before = carry, all = carry;
+    for (int w = 0; w < warps; ++w) {
+      if (w < warp) before += warp_part[w];
+      all += warp_part[w];
+    }
+    if (i < E) cnt[i] = before + s - v;
+    carry = all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) cnt[E] = carry;
+  __syncthreads();
+}
+
+// One cluster sorts all pairs; see the top of the file.  Shared: hist[warps][E], then total[E + 1].
+__global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads)
+    moe_plan_kernel(const int32_t* __restrict__ indices, int64_t pairs, int E, int32_t* __restrict__ offsets,
+                    int32_t* __restrict__ rows) {
+  extern __shared__ int plan_smem[];
+  __shared__ int warp_part[kPlanWarps];
+  int* hist = plan_smem;                 // [kPlanWarps][E]: counts, then next row of (warp, expert)
+  int* total = hist + kPlanWarps * E;    // [E + 1]: this CTA's counts; peers read them
+  int* start = total + E + 1;            // [E + 1]: offsets of the experts
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t rank = cluster_ctarank();
+  for (int i = threadIdx.x; i < kPlanWarps * E; i += kPlanThreads) hist[i] = 0;
+  __syncthreads();
+  // contiguous parts, a multiple of 32 pairs for each warp
+  const int64_t per_warp = ((pairs + kPlanCtas * kPlanWarps - 1) / (kPlanCtas * kPlanWarps) + 31) / 32 * 32;
+  const int64_t lo = ((int64_t)rank * kPlanWarps + warp) * per_warp;
+  const int64_t hi = lo + per_warp < pairs ? lo + per_warp : pairs;
+  int* mine = hist + warp * E;
+  for (int64_t i = lo + lane; i - lane < hi; i += 32) {
+    const int e = i < hi ? indices[i] : -1;
+    if (e >= 0 && e < E) atomicAdd(&mine[e], 1);  // a count: the order does not matter
+  }
+  __syncthreads();
+  // per expert: exclusive sums over the warps, the CTA's total
+  for (int e = threadIdx.x; e < E; e += kPlanThreads) {
+    int s = 0;
+    for (int w = 0; w < kPlanWarps; ++w) {
+      const int c = hist[w * E + e];
+      hist[w * E + e] = s;
+      s += c;
+    }
+    total[e] = s;
+  }
+  cluster_sync();
+  for (int e = threadIdx.x; e < E; e += kPlanThreads) {
+    int before = 0, all = 0;
+    for (uint32_t r = 0; r < kPlanCtas; ++r) {
+      int c;
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c) : "r"(mapa_shared(smem_u32(&total[e]), r)) : "memory");
+      if (r < rank) before += c;
+      all += c;
+    }
+    start[e] = all;
+    for (int w = 0; w < kPlanWarps; ++w) hist[w * E + e] += before;
+  }
+  __syncthreads();
+  block_exclusive_scan(start, E, warp_part);
+  if (rank == 0)
+    for (int e = threadIdx.x; e <= E; e += kPlanThreads) offsets[e] = start[e];
+  // ranks, in the order of the pairs
+  for (int64_t i = lo + lane; i - lane < hi; i += 32) {
+    const int e0 = i < hi ? indices[i] : -1;
+    const int e = e0 >= 0 && e0 < E ? e0 : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, e);
+    int row = -1;
+    if (e >= 0) row = start[e] + mine[e] + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (e >= 0 && lane == 31 - __clz(same)) mine[e] += __popc(same);
+    __syncwarp();
+    if (i < hi) rows[i] = row;
+  }
+  cluster_sync();  // peers may still read this CTA's totals
+}
+
+// 16 consecutive values of x as fp32 pairs.
+__device__ __forceinline__ void load16(const DispatchParams& p, int64_t at, int64_t col, float (&v)[16]) {
+  if (p.vec && col + 16 <= p.cols) {
+    if (p.x_f32) {
+      const float4* s = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + at + col);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 f = __ldcs(s + i);
+        v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
+      }
+    } else {
+      const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + at + col);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint4 u = __ldcs(s + i);
+        v[8 * i] = bf16lo(u.x), v[8 * i + 1] = bf16hi(u.x), v[8 * i + 2] = bf16lo(u.y), v[8 * i + 3] = bf16hi(u.y);
+        v[8 * i + 4] = bf16lo(u.z), v[8 * i + 5] = bf16hi(u.z), v[8 * i + 6] = bf16lo(u.w), v[8 * i + 7] = bf16hi(u.w);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    v[i] = col + i < p.cols ? load_f32(p.x, at + col + i, p.x_f32 ? B2X_F32 : B2X_BF16) : 0.0f;
+}
+
+template <int FP8>
+__device__ __forceinline__ void store16(const DispatchParams& p, const float (&v)[16], float inv, int64_t col,
+                                        const int* row, int k) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = quant4<FP8>(make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]), inv);
+  const bool whole = p.vec && col + 16 <= p.cols;
+  for (int j = 0; j < k; ++j) {
+    if (row[j] < 0) continue;
+    uint8_t* q = p.q + (int64_t)row[j] * p.ld_q + col;
+    if (whole) {
+      __stcs(reinterpret_cast<uint4*>(q), make_uint4(w[0], w[1], w[2], w[3]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (col + i < p.cols) q[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+    }
+  }
+}
+
+// One CTA per token.  NV: 16-value pieces that a thread holds in registers (cols <= kRowThreads * 16 * NV); NV = 0:
+// longer rows, read a second time (from L2) for the cast.
+template <int NV, int FP8>
+__global__ void __launch_bounds__(kRowThreads) moe_dispatch_kernel(const DispatchParams p) {
+  extern __shared__ int row_smem[];  // fused: cnt[E + 1]; always: row[k]
+  __shared__ int warp_part[kRowThreads / 32];
+  __shared__ float warp_max_[kRowThreads / 32];
+  const int64_t t = blockIdx.x;
+  int* row = row_smem;
+  int* cnt = row_smem + p.k;
+  const int64_t at = t * p.ld_x;
+  float v[NV ? NV : 1][16];
+  float amax = 0.0f;
+  // the row's loads are issued before the ranking
+  if (NV) {
+#pragma unroll
+    for (int n = 0; n < NV; ++n) load16(p, at, (int64_t)(n * kRowThreads + threadIdx.x) * 16, v[n]);
+  }
+  if (p.fused) {
+    const int pairs = (int)(p.tokens * p.k), own = (int)(t * p.k);
+    for (int e = threadIdx.x; e < p.E; e += kRowThreads) cnt[e] = 0;
+    for (int j = threadIdx.x; j < p.k; j += kRowThreads) row[j] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < pairs; i += kRowThreads) {
+      const int e = p.indices[i];
+      if (e >= 0 && e < p.E) atomicAdd(&cnt[e], 1);
+      for (int j = 0; j < p.k; ++j)  // pairs before this token's j-th that go to the same expert
+        if (i < own + j && e == __ldg(p.indices + own + j)) atomicAdd(&row[j], 1);
+    }
+    __syncthreads();
+    block_exclusive_scan(cnt, p.E, warp_part);
+    for (int j = threadIdx.x; j < p.k; j += kRowThreads) {
+      const int e = __ldg(p.indices + own + j);
+      const int r = e >= 0 && e < p.E ? row[j] + cnt[e] : -1;
+      row[j] = r;
+      p.rows[own + j] = r;
+    }
+    if (t == 0)
+      for (int e = threadIdx.x; e <= p.E; e += kRowThreads) p.offsets[e] = cnt[e];
+  } else {
+    for (int j = threadIdx.x; j < p.k; j += kRowThreads) row[j] = p.rows[t * p.k + j];
+  }
+  float s;
+  if (!p.given) {
+    if (NV) {
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) amax = absmax_xs(amax, v[n][i]);
+    } else {
+      for (int64_t c = (int64_t)threadIdx.x * 16; c < p.cols; c += kRowThreads * 16) {
+        load16(p, at, c, v[0]);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) amax = absmax_xs(amax, v[0][i]);
+      }
+    }
+    amax = fabsf(amax);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if ((threadIdx.x & 31) == 0) warp_max_[threadIdx.x >> 5] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kRowThreads / 32; ++w) amax = fmaxf(amax, warp_max_[w]);
+    s = __fdiv_rn(amax, Fp8Traits<FP8>::kMax);
+  } else {
+    __syncthreads();
+    s = __ldg(p.given);
+  }
+  const float inv = s == 0.0f ? 0.0f : __fdiv_rn(1.0f, s);
+  if (!p.given)
+    for (int j = threadIdx.x; j < p.k; j += kRowThreads)
+      if (row[j] >= 0) p.scale[row[j]] = s;
+  if (NV) {
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int64_t c = (int64_t)(n * kRowThreads + threadIdx.x) * 16;
+      if (c < p.cols) store16<FP8>(p, v[n], inv, c, row, p.k);
+    }
+  } else {
+    for (int64_t c = (int64_t)threadIdx.x * 16; c < p.cols; c += kRowThreads * 16) {
+      load16(p, at, c, v[0]);
+      store16<FP8>(p, v[0], inv, c, row, p.k);
+    }
+  }
+}
+
+template <int FP8>
+static void launch_dispatch_rows(const DispatchParams& p, size_t smem, cudaStream_t st) {
+  const int64_t per = (p.cols + kRowThreads * 16 - 1) / (kRowThreads * 16);
+  const unsigned grid = (unsigned)p.tokens;
+  if (per <= 1) moe_dispatch_kernel<1, FP8><<<grid, kRowThreads, smem, st>>>(p);
+  else if (per <= 2) moe_dispatch_kernel<2, FP8><<<grid, kRowThreads, smem, st>>>(p);
+  else if (per <= 4) moe_dispatch_kernel<4, FP8><<<grid, kRowThreads, smem, st>>>(p);
+  else moe_dispatch_kernel<0, FP8><<<grid, kRowThreads, smem, st>>>(p);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- combine
+
+struct CombineParams {
+  const void* y;
+  int64_t y_rows, ld_y;
+  const int32_t* rows;
+  const float* weights;
+  int64_t tokens, cols;
+  int k;
+  const void* residual;
+  int64_t ld_res;
+  void* out;  // combine: out; backward: d_y
+  int64_t ld_out;
+  const void* grad;
+  int64_t ld_grad;
+  float* d_weights;
+};
+
+// V consecutive values as loaded (V * sizeof(T) = 16 bytes, or one value).
+template <typename T, int V>
+struct Piece {
+  T e[V];
+};
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) {
+  if constexpr (sizeof(T) == 4)
+    return v;
+  else if constexpr (__is_same(T, __half))
+    return __half2float(v);
+  else
+    return __bfloat162float(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_f32(float f) {
+  if constexpr (sizeof(T) == 4)
+    return f;
+  else if constexpr (__is_same(T, __half))
+    return __float2half_rn(f);
+  else
+    return __float2bfloat16_rn(f);
+}
+template <typename T, int V>
+__device__ __forceinline__ Piece<T, V> load_piece(const T* p) {
+  if constexpr (V == 1) {
+    return Piece<T, V>{{*p}};
+  } else {
+    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
+    Piece<T, V> r;
+    memcpy(&r, &u, 16);
+    return r;
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_piece(T* p, const Piece<T, V>& v) {
+  if constexpr (V == 1) {
+    *p = v.e[0];
+  } else {
+    uint4 u;
+    memcpy(&u, &v, 16);
+    __stcs(reinterpret_cast<uint4*>(p), u);
+  }
+}
+
+// One CTA per (token, kRowThreads * V columns).
+template <typename T, int V>
+__global__ void __launch_bounds__(kRowThreads) moe_combine_kernel(const CombineParams p) {
+  const uint32_t per = (uint32_t)((p.cols + kRowThreads * V - 1) / (kRowThreads * V));  // CTAs of a token: < 2^31 in all
+  const int64_t t = blockIdx.x / per;
+  const int64_t c = ((int64_t)(blockIdx.x % per) * kRowThreads + threadIdx.x) * V;
+  if (c >= p.cols) return;
+  const T* y = reinterpret_cast<const T*>(p.y);
+  float acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+  constexpr int U = 8;  // rows in flight
+  for (int j0 = 0; j0 < p.k; j0 += U) {
+    Piece<T, V> v[U];
+    float w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = j0 + u < p.k ? __ldg(p.rows + t * p.k + j0 + u) : -1;
+      const bool in = r >= 0 && r < p.y_rows;
+      w[u] = in ? (p.weights ? __ldg(p.weights + t * p.k + j0 + u) : 1.0f) : 0.0f;
+      if (in)
+        v[u] = load_piece<T, V>(y + r * p.ld_y + c);
+      else
+        v[u] = Piece<T, V>{};
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = fmaf(w[u], to_f32(v[u].e[i]), acc[i]);
+  }
+  if (p.residual) {
+    const Piece<T, V> r = load_piece<T, V>(reinterpret_cast<const T*>(p.residual) + t * p.ld_res + c);
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] += to_f32(r.e[i]);
+  }
+  Piece<T, V> o;
+#pragma unroll
+  for (int i = 0; i < V; ++i) o.e[i] = from_f32<T>(acc[i]);
+  store_piece<T, V>(reinterpret_cast<T*>(p.out) + t * p.ld_out + c, o);
+}
+
+// One CTA per token; KC slots at a time (their dot products stay in registers).
+template <typename T, int V, int KC>
+__global__ void __launch_bounds__(kRowThreads) moe_combine_backward_kernel(const CombineParams p) {
+  __shared__ float part[kRowThreads / 32][KC];
+  const int64_t t = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const T* y = reinterpret_cast<const T*>(p.y);
+  const T* g = reinterpret_cast<const T*>(p.grad) + t * p.ld_grad;
+  T* dy = reinterpret_cast<T*>(p.out);
+  for (int j0 = 0; j0 < p.k; j0 += KC) {
+    int64_t r[KC];
+    float w[KC], dot[KC];
+#pragma unroll
+    for (int u = 0; u < KC; ++u) {
+      r[u] = j0 + u < p.k ? __ldg(p.rows + t * p.k + j0 + u) : -1;
+      if (r[u] >= p.y_rows) r[u] = -1;
+      w[u] = j0 + u < p.k ? __ldg(p.weights + t * p.k + j0 + u) : 0.0f;
+      dot[u] = 0.0f;
+    }
+    for (int64_t c = (int64_t)threadIdx.x * V; c < p.cols; c += kRowThreads * V) {
+      Piece<T, V> v[KC];
+#pragma unroll
+      for (int u = 0; u < KC; ++u)
+        if (r[u] >= 0)
+          v[u] = load_piece<T, V>(y + r[u] * p.ld_y + c);
+        else
+          v[u] = Piece<T, V>{};
+      const Piece<T, V> gv = load_piece<T, V>(g + c);
+      float gf[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) gf[i] = to_f32(gv.e[i]);
+#pragma unroll
+      for (int u = 0; u < KC; ++u) {
+        if (r[u] < 0) continue;
+        Piece<T, V> o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          dot[u] = fmaf(gf[i], to_f32(v[u].e[i]), dot[u]);
+          o.e[i] = from_f32<T>(w[u] * gf[i]);
+        }
+        store_piece<T, V>(dy + r[u] * p.ld_out + c, o);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < KC; ++u) {
+#pragma unroll
+      for (int o = 16; o; o >>= 1) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], o);
+      if (lane == 0) part[warp][u] = dot[u];
+    }
+    __syncthreads();
+    if (threadIdx.x < KC && j0 + (int)threadIdx.x < p.k) {
+      float s = 0.0f;
+#pragma unroll
+      for (int q = 0; q < kRowThreads / 32; ++q) s += part[q][threadIdx.x];
+      p.d_weights[t * p.k + j0 + threadIdx.x] = s;
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, int BACKWARD>
+static cudaError_t launch_combine_t(const CombineParams& p, bool vec, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  if constexpr (BACKWARD) {
+    const unsigned grid = (unsigned)p.tokens;
+    if (vec)
+      moe_combine_backward_kernel<T, V, 8><<<grid, kRowThreads, 0, st>>>(p);
+    else
+      moe_combine_backward_kernel<T, 1, 8><<<grid, kRowThreads, 0, st>>>(p);
+  } else {
+    const int v = vec ? V : 1;
+    const int64_t per = (p.cols + kRowThreads * v - 1) / (kRowThreads * v);
+    const unsigned grid = (unsigned)(p.tokens * per);
+    if (vec)
+      moe_combine_kernel<T, V><<<grid, kRowThreads, 0, st>>>(p);
+    else
+      moe_combine_kernel<T, 1><<<grid, kRowThreads, 0, st>>>(p);
+  }
+  note_launch(1);
+  return cudaGetLastError();
+}
+
+template <int BACKWARD>
+static cudaError_t launch_combine(const CombineParams& p, b2x_dtype type, bool vec, cudaStream_t st) {
+  if (type == B2X_F32) return launch_combine_t<float, BACKWARD>(p, vec, st);
+  if (type == B2X_F16) return launch_combine_t<__half, BACKWARD>(p, vec, st);
+  return launch_combine_t<__nv_bfloat16, BACKWARD>(p, vec, st);
+}
+
+// Rows of `elem`-byte values that start on 16-byte boundaries.
+static bool rows_aligned(const void* p, int64_t ld, int elem) {
+  return ((uintptr_t)p % 16) == 0 && (ld * elem) % 16 == 0;
+}
+
+static bool is_float_type(b2x_dtype t) { return t == B2X_F32 || t == B2X_BF16 || t == B2X_F16; }
+
+}  // namespace b2x
+
+extern "C" B2X_API b2x_status b2x_moe_dispatch(const b2x_moe_dispatch_args* a, void* stream) {
+  using namespace b2x;
+  t_err[0] = 0;
+  if (!a) return fail(B2X_ERR_INVALID_ARG, "b2x_moe_dispatch: args is NULL");
+  if (a->x_type != B2X_F32 && a->x_type != B2X_BF16)
+    return fail(B2X_ERR_UNSUPPORTED, "b2x_moe_dispatch: x must be fp32 or bf16");
+  if (!is_fp8(a->q_type)) return fail(B2X_ERR_UNSUPPORTED, "b2x_moe_dispatch: q must be e4m3 or e5m2");
+  if (a->tokens < 0 || a->cols < 0 || a->ld_x < a->cols || a->ld_q < a->cols || a->top_k < 1 || a->experts < 1)
+    return fail(B2X_ERR_INVALID_ARG, "b2x_moe_dispatch: bad shape (tokens %lld, cols %lld, top_k %d, experts %lld)",
+                (long long)a->tokens, (long long)a->cols, a->top_k, (long long)a->experts);
+  if (a->experts > 1024 || a->top_k > 1024)
+    return fail(B2X_ERR_UNSUPPORTED, "b2x_moe_dispatch: at most 1024 experts and top_k 1024");
+  if (a->tokens * a->top_k >= (1LL << 31)) return fail(B2X_ERR_UNSUPPORTED, "b2x_moe_dispatch: tokens * top_k must be < 2^31");
+  if (!a->offsets) return fail(B2X_ERR_INVALID_ARG, "b2x_moe_dispatch: NULL offsets");
+  cudaStream_t st = (cudaStream_t)stream;
+  if (a->tokens == 0) {
+    cudaError_t e = cudaMemsetAsync(a->offsets, 0, (size_t)(a->experts + 1) * 4, st);
+    return e == cudaSuccess ? B2X_OK : cuda_fail(e, "b2x_moe_dispatch: clearing offsets");
+  }
+  if (!a->indices || !a->rows || (a->cols > 0 && (!a->x || !a->q)) || (!a->given && !a->scale))
+    return fail(B2X_ERR_INVALID_ARG, "b2x_moe_dispatch: NULL pointer");
+  DispatchParams p{};
+  p.x = a->x;
+  p.x_f32 = a->x_type == B2X_F32;
+  p.tokens = a->tokens;
+  p.cols = a->cols;
+  p.ld_x = a->ld_x;
+  p.indices = a->indices;
+  p.k = a->top_k;
+  p.E = (int)a->experts;
+  p.q = reinterpret_cast<uint8_t*>(a->q);
+  p.ld_q = a->ld_q;
+  p.scale = a->scale;
+  p.given = a->given;
+  p.offsets = a->offsets;
+  p.rows = a->rows;
+  const int64_t pairs = a->tokens * a->top_k;
+  p.fused = pairs <= kFusedPairs;
+  p.vec = rows_aligned(a->x, a->ld_x, p.x_f32 ? 4 : 2) && rows_aligned(a->q, a->ld_q, 1);
+  if (!p.fused) {
+    const int smem = (kPlanWarps * p.E + 2 * (p.E + 1)) * 4;
+    cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(moe_plan_kernel), smem);
+    if (e != cudaSuccess) return cuda_fail(e, "b2x_moe_dispatch: shared memory");
+    moe_plan_kernel<<<kPlanCtas, kPlanThreads, smem, st>>>(a->indices, pairs, p.E, a->offsets, a->rows);
+    note_launch(1);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "b2x_moe_dispatch launch (plan)");
+  }
+  const size_t smem = (size_t)(p.k + (p.fused ? p.E + 1 : 0)) * 4;
+  if (a->q_type == B2X_E5M2)
+    launch_dispatch_rows<1>(p, smem, st);
+  else
+    launch_dispatch_rows<0>(p, smem, st);
+  note_launch(1);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? B2X_OK : cuda_fail(e, "b2x_moe_dispatch launch");
+}
+
+extern "C" B2X_API b2x_status b2x_moe_combine(const void* y, int64_t y_rows, int64_t ld_y, const int32_t* rows,
+                                              const float* weights, int64_t tokens, int top_k, int64_t cols,
+                                              const void* residual, int64_t ld_residual, void* out, int64_t ld_out,
+                                              b2x_dtype type, void* stream) {
+  using namespace b2x;
+  t_err[0] = 0;
+  if (!is_float_type(type)) return fail(B2X_ERR_UNSUPPORTED, "b2x_moe_combine: type must be fp32, bf16 or fp16");
+  if (tokens < 0 || cols < 0 || y_rows < 0 || top_k < 1 || ld_y < cols || ld_out < cols || (residual && ld_residual < cols))
+    return fail(B2X_ERR_INVALID_ARG, "b2x_moe_combine: bad shape or row stride");
+  if (tokens == 0 || cols == 0) return B2X_OK;
+  if ((y_rows > 0 && !y) || !rows || !out) return fail(B2X_ERR_INVALID_ARG, "b2x_moe_combine: NULL pointer");
+  CombineParams p{};
+  p.y = y;
+  p.y_rows = y_rows;
+  p.ld_y = ld_y;
+  p.rows = rows;
+  p.weights = weights;
+  p.tokens = tokens;
+  p.cols = cols;
+  p.k = top_k;
+  p.residual = residual;
+  p.ld_res = ld_residual;
+  p.out = out;
+  p.ld_out = ld_out;
+  const int elem = type == B2X_F32 ? 4 : 2;
+  const bool vec = cols % (16 / elem) == 0 && rows_aligned(y, ld_y, elem) && rows_aligned(out, ld_out, elem) &&
+                   (!residual || rows_aligned(residual, ld_residual, elem));
+  const int64_t ctas = tokens * ((cols + kRowThreads - 1) / kRowThreads);
+  if (ctas >= (1LL << 31)) return fail(B2X_ERR_UNSUPPORTED, "b2x_moe_combine: tokens * cols / 128 must be < 2^31");
+  cudaError_t e = launch_combine<0>(p, type, vec, (cudaStream_t)stream);
+  return e == cudaSuccess ? B2X_OK : cuda_fail(e, "b2x_moe_combine launch");
+}
+
+extern "C" B2X_API b2x_status b2x_moe_combine_backward(const void* grad, int64_t ld_grad, const void* y, int64_t y_rows,
+                                                       int64_t ld_y, const int32_t* rows, const float* weights,
+                                                       int64_t tokens, int top_k, int64_t cols, void* d_y,
+                                                       int64_t ld_d_y, float* d_weights, b2x_dtype type, void* stream) {
+  using namespace b2x;
+  t_err[0] = 0;
+  if (!is_float_type(type)) return fail(B2X_ERR_UNSUPPORTED, "b2x_moe_combine_backward: type must be fp32, bf16 or fp16");
+  if (tokens < 0 || cols < 0 || y_rows < 0 || top_k < 1 || ld_y < cols || ld_grad < cols || ld_d_y < cols)
+    return fail(B2X_ERR_INVALID_ARG, "b2x_moe_combine_backward: bad shape or row stride");
+  if (tokens >= (1LL << 31)) return fail(B2X_ERR_UNSUPPORTED, "b2x_moe_combine_backward: tokens must be < 2^31");
+  if (tokens == 0) return B2X_OK;
+  if (!rows || !weights || !d_weights || (cols > 0 && (!grad || (y_rows > 0 && (!y || !d_y)))))
+    return fail(B2X_ERR_INVALID_ARG, "b2x_moe_combine_backward: NULL pointer");
+  CombineParams p{};
+  p.y = y;
+  p.y_rows = y_rows;
+  p.ld_y = ld_y;
+  p.rows = rows;
+  p.weights = weights;
+  p.tokens = tokens;
+  p.cols = cols;
+  p.k = top_k;
+  p.out = d_y;
+  p.ld_out = ld_d_y;
+  p.grad = grad;
+  p.ld_grad = ld_grad;
+  p.d_weights = d_weights;
+  const int elem = type == B2X_F32 ? 4 : 2;
+  const bool vec = cols % (16 / elem) == 0 && rows_aligned(y, ld_y, elem) && rows_aligned(d_y, ld_d_y, elem) &&
+                   rows_aligned(grad, ld_grad, elem);
+  cudaError_t e = launch_combine<1>(p, type, vec, (cudaStream_t)stream);
+  return e == cudaSuccess ? B2X_OK : cuda_fail(e, "b2x_moe_combine_backward launch");
+}
