@@ -84,6 +84,9 @@ LINEAR = [  # M, N, K, activation, bias, residual, out, pre, layout
     (700, 1032, 256, "silu", BF, True, HF, True, "nk"),
     (1025, 2304, 1040, "gelu_tanh", F32, True, BF, True, "nk"),
     (2000, 3968, 512, "relu", F32, True, BF, False, "kn"),
+    (4500, 1100, 272, "gelu", F32, True, BF, True, "nk"),     # more than one band of token tiles, half a weight tile over
+    (257, 19000, 128, "silu", None, False, HF, False, "nk"),
+    (5000, 1039, 300, "gelu_tanh", BF, True, HF, True, "nk"),
 ]
 
 
@@ -547,6 +550,11 @@ EXPERTS = [  # counts, N, K, layout, rows behind
     ([0, 0, 0], 128, 128, "nk", 4),
     ([513, 511, 256, 2, 1000], 520, 1024, "nk", 5),
     ([9, 8], 40, 100, "nk", 0),
+    ([5] * 70, 1100, 384, "nk", 1),
+    ([1, 0, 300, 33, 513] * 14, 640, 144, "nk", 3),
+    ([0, 70, 17, 256, 31, 1, 257] * 10, 528, 272, "kn", 3),
+    ([0] * 999 + [4200], 1300, 128, "nk", 6),
+    ([3] * 1000, 300, 256, "nk", 0),
 ]
 
 
@@ -634,7 +642,8 @@ def check_codes(q, ref, err, dtype):
 
 
 @pytest.mark.parametrize("counts,I,K,behind", [([1], 128, 128, 0), ([3, 0, 1, 9], 256, 400, 2), ([40, 64, 0, 21], 128, 272, 0),
-                                               ([300, 129, 1], 384, 512, 5), ([1024, 700, 0, 513], 256, 1024, 1)])
+                                               ([300, 129, 1], 384, 512, 5), ([1024, 700, 0, 513], 256, 1024, 1),
+                                               ([7, 0, 290, 1] * 20, 384, 272, 4)])
 @pytest.mark.parametrize("dtype", [E4, E5])
 def test_moe_gemm_swiglu(counts, I, K, behind, dtype):
     import b2x

@@ -232,6 +232,283 @@ __global__ void __launch_bounds__(kTkThreads, 2)
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------- pairs
+//
+// fp8_gemm_tokens_pair_kernel: the same products for many tokens, persistent, on CTA pairs (cta_group::2): a pair owns
+// 256 weight rows x up to 256 tokens; CTA r holds weight rows 128 r .. 128 r + 127 of the tile in its TMEM and loads
+// those rows and half of the tokens, 32 KB per CTA and K block where a single CTA's 128 x 256 tile needs 48 KB (no
+// multicast).  The tile is as wide as its tokens need, in steps of 32.  Two accumulators let the two epilogue
+// warpgroups of a CTA work behind the next tile's MMAs.  Roles as in fp8_gemm_pair.cu: warp 0 loads, warp 1 of the even
+// CTA issues the MMAs, warp 2 allocates TMEM, warps 4-11 finish tiles.  The units are found by every role itself: a warp
+// keeps 32 experts' ranges in its lanes (TokCursor) and moves on in the order of the units.
+
+constexpr int kTpTokens = 256;    // tokens per unit
+constexpr int kTpBox = 64;        // tokens per load
+constexpr int kTpChunk = 16;      // tokens per epilogue step
+constexpr int kTpBand = 16;       // token tiles whose X stays in L2 while the weight tiles go by
+
+template <int STAGES>
+struct TpSmem {
+  static constexpr int kWBytes = kTkRows * kBK;               // 16 KB
+  static constexpr int kXBytes = (kTpTokens / 2) * kBK;       // 16 KB
+  static constexpr int kStageBytes = kWBytes + kXBytes;
+  static constexpr int kCBytes = 2 * kTpChunk * kTkRows * 4;  // two steps of 8 KB per warpgroup
+  static constexpr int kXOff = STAGES * kWBytes;
+  static constexpr int kCOff = STAGES * kStageBytes;
+  static constexpr int kBarOff = kCOff + 2 * kCBytes;
+  static constexpr int kAlloc = kBarOff + (2 * STAGES + 5) * 8 + 16 + 1024;
+};
+constexpr int kTpStages = (kMaxDynSmem - 2 * TpSmem<1>::kCBytes - 1024 - 256) / TpSmem<1>::kStageBytes;
+
+// Walks the units in rising order; all lanes of a warp together.
+struct TokCursor {
+  int base, carry, total, s, mt;  // experts base .. base + 31; units before them, in them; lane's inclusive sum, token tiles
+  int64_t lo, rows;               // lane's range
+};
+__device__ __forceinline__ void tok_chunk(const TokParams& p, TokCursor& c, int n2, int lane) {
+  c.lo = c.rows = 0;
+  if (!p.offsets) {
+    if (c.base + lane == 0) c.rows = p.rows;
+  } else if (c.base + lane < p.E) {
+    int64_t hi;
+    tok_range(p, c.base + lane, c.lo, hi);
+    c.rows = hi - c.lo;
+  }
+  c.mt = (int)((c.rows + kTpTokens - 1) / kTpTokens);
+  c.s = c.mt * n2;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, c.s, o);
+    if (lane >= o) c.s += v;
+  }
+  c.total = __shfl_sync(0xffffffffu, c.s, 31);
+}
+// The unit, or cnt = 0 past the last one.  nt: index of the 256-row weight tile.
+__device__ __forceinline__ TokUnit tok_seek(const TokParams& p, TokCursor& c, int unit, int n2, int lane) {
+  TokUnit u{0, 0, 0, 0};
+  while (unit >= c.carry + c.total) {
+    c.base += 32;
+    if (c.base >= p.E) return u;
+    c.carry += c.total;
+    tok_chunk(p, c, n2, lane);
+  }
+  const int src = __ffs(__ballot_sync(0xffffffffu, unit < c.carry + c.s)) - 1;
+  const int mt = __shfl_sync(0xffffffffu, c.mt, src);
+  const int local = unit - c.carry - (__shfl_sync(0xffffffffu, c.s, src) - mt * n2);
+  const int64_t lo = __shfl_sync(0xffffffffu, c.lo, src), rows = __shfl_sync(0xffffffffu, c.rows, src);
+  const int band = local / (kTpBand * n2);
+  const int width = min(kTpBand, mt - band * kTpBand);
+  const int r = local - band * kTpBand * n2;
+  const int m = band * kTpBand + r % width;
+  u.e = c.base + src;
+  u.nt = r / width;
+  u.row0 = lo + (int64_t)m * kTpTokens;
+  u.cnt = (int)min((int64_t)kTpTokens, rows - (int64_t)m * kTpTokens);
+  return u;
+}
+
+template <int W_KIND>
+__device__ __forceinline__ void tok_load_w_pair(const TokParams& p, void* dst, const CUtensorMap* m, uint32_t bar, int kb,
+                                                int e, int nt, uint64_t pol) {
+  if constexpr (W_KIND == 0)
+    tma_load_3d_pair(dst, m, bar, kb * kBK, nt * kTkRows, e, pol);
+  else if constexpr (W_KIND == 1)
+    tma_load_3d_pair(dst, m, bar, nt * kTkRows, kb * kBK, e, pol);
+  else
+    tma_load_5d_pair(dst, m, bar, kb * kBK, 0, 0, (nt & 1) * 4, e * (p.N / 256) + (nt >> 1), pol);
+}
+
+template <int W_KIND>
+__global__ void __launch_bounds__(kThreads, 1)
+    fp8_gemm_tokens_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                                const TokParams p) {
+  constexpr int STAGES = kTpStages;
+  using L = TpSmem<STAGES>;
+  static_assert(L::kAlloc <= kMaxDynSmem, "shared memory plan exceeds the opt-in limit");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* mma_done = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 2);
+    }
+    mbar_init(mma_done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+  }
+  if (warp == 2) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int n2 = (p.n_tiles + 1) / 2;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  TokCursor cur{0, 0, 0, 0, 0, 0, 0};
+  if (warp < 2 || warp >= kEpiWarp0) tok_chunk(p, cur, n2, lane);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ loads (both CTAs)
+    const uint64_t pol_w = l2_policy(p.l2_w), pol_x = policy_evict_last();
+    int stage = 0;
+    uint32_t phase = 0, issued = 0, pend = 0;  // pend: bit s = phase of stage s's last load
+    bool ok = true;
+    for (int unit = first; ok; unit += step) {
+      const TokUnit u = tok_seek(p, cur, unit, n2, lane);
+      if (u.cnt == 0) break;
+      if (lane == 0) {
+        const int half = (u.cnt + 31) / 32 * 16;  // tokens per CTA
+        const int boxes = (half + kTpBox - 1) / kTpBox;
+        const int x0 = (int)u.row0 + (int)rank * half;
+        for (int kb = 0; kb < p.k_tiles; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, kStatusTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);
+          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * (L::kWBytes + boxes * kTpBox * kBK));
+          uint8_t* sx = smem + L::kXOff + stage * L::kXBytes;
+          tok_load_w_pair<W_KIND>(p, smem + stage * L::kWBytes, &tmW, bar, kb, u.e, 2 * u.nt + (int)rank, pol_w);
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d_pair(sx + b * kTpBox * kBK, &tmX, bar, kb * kBK, x0 + b * kTpBox, pol_x);
+          issued |= 1u << stage;
+          pend = (pend & ~(1u << stage)) | (phase << stage);
+          if (++stage == STAGES) stage = 0, phase ^= 1;
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+    }
+    // the even CTA's full barriers count both CTAs' loads: none is in flight once they have completed
+    if (leader && lane == 0)
+      for (int s = 0; s < STAGES; ++s)
+        if (issued & (1u << s)) {
+          volatile int no_abort = 0;
+          mbar_wait(&full[s], (pend >> s) & 1, &no_abort, kStatusTimeoutProducer);
+        }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMAs (even CTA)
+    if (leader) {
+      int stage = 0, local = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int unit = first; ok; unit += step, ++local) {
+        const TokUnit u = tok_seek(p, cur, unit, n2, lane);
+        if (u.cnt == 0) break;
+        if (lane == 0) {
+          const int buf = local & 1;
+          const uint32_t idesc = p.idesc | ((uint32_t)((u.cnt + 31) / 32 * 4) << 17);
+          ok = mbar_wait(&tempty[buf], ((local >> 1) & 1) ^ 1, abort_flag, kStatusTimeoutMma);
+          tc_fence_after();
+          const uint32_t d = tmem_base + buf * kTpTokens;
+          for (int kb = 0; ok && kb < p.k_tiles; ++kb) {
+            if (!mbar_wait(&full[stage], phase, abort_flag, kStatusTimeoutMma)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t w = smem_u32(smem + stage * L::kWBytes), x = smem_u32(smem + L::kXOff + stage * L::kXBytes);
+#pragma unroll
+            for (int k = 0; k < kBK / 32; ++k)
+              mma_f8f6f4_pair(d,
+                              W_KIND == 1 ? smem_desc_sw128(w + k * 32 * 128, 128 * kBK, 1024)
+                                          : smem_desc_sw128(w + k * 32, 16, 1024),
+                              smem_desc_sw128(x + k * 32, 16, 1024), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+            mma_commit_pair_mc(&empty[stage], 0x3);
+            if (++stage == STAGES) stage = 0, phase ^= 1;
+          }
+          if (ok) mma_commit_pair_mc(&tfull[buf], 0x3);
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      }
+      if (lane == 0) {
+        mma_commit_pair_mc(mma_done, 0x1);
+        volatile int no_abort = 0;
+        mbar_wait(mma_done, 0, &no_abort, kStatusTimeoutMma);
+      }
+    }
+  } else if (warp >= kEpiWarp0) {
+    // ------------------------------------------------------------ epilogue (both CTAs)
+    const int e = (warp - kEpiWarp0) >> 2, q = warp & 3;
+    const uint32_t bar_id = 1 + e;
+    const int wg_tid = threadIdx.x - (kEpiWarp0 + 4 * e) * 32;
+    float* stage_c = reinterpret_cast<float*>(smem + L::kCOff + e * L::kCBytes);
+    const uint32_t tempty_leader = mapa_shared(smem_u32(&tempty[e]), 0);
+    float inv = 0.0f, amax = 0.0f;
+    if constexpr (W_KIND == 2) {
+      const float hs = __ldg(p.h_scale);
+      inv = hs == 0.0f ? 0.0f : __fdiv_rn(1.0f, hs);
+    }
+    int local = 0;
+    for (int unit = first;; unit += step, ++local) {
+      const TokUnit u = tok_seek(p, cur, unit, n2, lane);
+      if (u.cnt == 0) break;
+      if ((local & 1) != e) continue;
+      const bool ok = mbar_wait(&tfull[e], (local >> 1) & 1, abort_flag, kStatusTimeoutEpilogue);
+      if (!wg_all(ok, bar_id)) break;
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + e * kTpTokens + ((uint32_t)(q * 32) << 16);
+      const int n0 = (2 * u.nt + (int)rank) * kTkRows;
+      const int chunks = (u.cnt + kTpChunk - 1) / kTpChunk;
+#pragma unroll 1
+      for (int c = 0; c < chunks; ++c) {
+        uint32_t v[kTpChunk];
+        tmem_ld_32x32b_x16(t_row + c * kTpChunk, v);
+        tmem_ld_wait();
+        tmem_regs_after_wait(v);
+        float* buf = stage_c + (c & 1) * kTpChunk * kTkRows;
+#pragma unroll
+        for (int i = 0; i < kTpChunk; ++i) buf[i * kTkRows + q * 32 + lane] = __uint_as_float(v[i]);
+        tc_fence_before();
+        // the other half of the staging was read before the barrier of the step before: one barrier a step
+        named_bar_sync(bar_id, 128);
+        if (c + 1 == chunks && wg_tid == 0) mbar_arrive_cluster_relaxed(tempty_leader);
+        auto fetch = [&](int m, int col) { return *reinterpret_cast<const float4*>(buf + m * kTkRows + col); };
+        const int cnt = min(kTpChunk, u.cnt - c * kTpChunk);
+        const int64_t row0 = u.row0 + c * kTpChunk;
+        if constexpr (W_KIND == 2)
+          tok_finish_swiglu(p, u.e, row0, n0, cnt, q, 4, lane, inv, amax, fetch);
+        else
+          tok_finish(p, u.e, row0, n0, cnt, q, 4, lane, fetch);
+      }
+      named_bar_sync(bar_id, 128);  // the next tile's first step writes the staging again
+    }
+    if constexpr (W_KIND == 2) {
+      if (p.h_amax) {
+        const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
+        if (lane == 0 && m) atomicMax(reinterpret_cast<unsigned*>(p.h_amax), m);
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();  // no CTA leaves while its peer may still use its shared memory or barriers
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
 struct TokLaunch {
   CUtensorMap tmW;
   TokParams p;
@@ -271,6 +548,30 @@ static cudaError_t launch_tokens_nt(const TokLaunch& g, const CUtensorMap& tmX, 
   return launch_tokens_t<NT, 2>(g, tmX, units, st);
 }
 
+template <int W_KIND>
+static cudaError_t launch_tokens_pair_t(const TokLaunch& g, const CUtensorMap& tmX, int64_t units, cudaStream_t st) {
+  using L = TpSmem<kTpStages>;
+  auto kern = fp8_gemm_tokens_pair_kernel<W_KIND>;
+  cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), L::kAlloc);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = L::kAlloc;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const int64_t pairs = std::min<int64_t>(units, g.num_sms / 2);
+  cfg.gridDim = dim3((unsigned)(2 * std::max<int64_t>(pairs, 1)), 1, 1);
+  e = cudaLaunchKernelEx(&cfg, kern, g.tmW, tmX, g.p);
+  note_launch(1);
+  return e;
+}
+
 // Experts that get a row when `rows` fall on E experts evenly: what the grid is planned for.
 static double expected_active(int64_t rows, int64_t E) { return (double)E * (1.0 - pow(1.0 - 1.0 / (double)E, (double)rows)); }
 
@@ -279,6 +580,27 @@ static b2x_status launch_tokens(TokLaunch& g, const char* who, cudaStream_t st) 
   const bool moe = p.offsets != nullptr;
   const double active = moe ? expected_active(p.rows, p.E) : 1.0;
   const double mean = (double)p.rows / active;
+  const double mean256 = ceil(mean / kTpTokens);
+  const double units2 = std::max(1.0, moe ? active * mean256 : mean256) * ((p.n_tiles + 1) / 2);
+  bool pair = units2 >= g.num_sms / 2;
+#ifdef B2X_TOK_FORCE
+  if (const char* f = getenv("B2X_TOK")) pair = f[0] == '2';
+#endif
+  if (pair) {
+    const int64_t most = (moe ? p.rows / kTpTokens + std::min<int64_t>(p.E, p.rows) : (p.rows + kTpTokens - 1) / kTpTokens) *
+                         ((p.n_tiles + 1) / 2);
+    if (most >= (1LL << 31)) return fail(B2X_ERR_UNSUPPORTED, "%s: too many tiles", who);
+    p.idesc = idesc_f8f6f4(g.w_fmt, g.x_fmt, g.w_kind == 1 ? 1 : 0, 0, 2 * kTkRows, 0);
+    p.l2_w = 0;
+    CUtensorMap tmX;
+    b2x_status s = encode_2d(&tmX, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.x, (uint64_t)p.K, (uint64_t)p.rows, (uint64_t)g.ld_x,
+                             128, kTpBox, CU_TENSOR_MAP_SWIZZLE_128B, "x");
+    if (s != B2X_OK) return s;
+    cudaError_t e = g.w_kind == 0   ? launch_tokens_pair_t<0>(g, tmX, most, st)
+                    : g.w_kind == 1 ? launch_tokens_pair_t<1>(g, tmX, most, st)
+                                    : launch_tokens_pair_t<2>(g, tmX, most, st);
+    return e == cudaSuccess ? B2X_OK : cuda_fail(e, who);
+  }
   // Token tile: the mean expert fits with room for an uneven spread.
   int nt = 128;
   if (mean <= (moe ? 10 : 16)) nt = 16;
