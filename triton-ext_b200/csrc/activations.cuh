@@ -44,24 +44,25 @@ __device__ __forceinline__ float act_slope(float x) {
   return 1.0f;
 }
 
-// Four values at once with the activation chosen at run time (uniform over the grid).
-__device__ __forceinline__ void act4(int act, float (&v)[4]) {
+// Values with the activation chosen at run time (uniform over the grid).
+template <int N>
+__device__ __forceinline__ void act_all(int act, float (&v)[N]) {
   switch (act) {
     case B2X_ACT_RELU:
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = act_fwd<B2X_ACT_RELU>(v[i]);
+      for (int i = 0; i < N; ++i) v[i] = act_fwd<B2X_ACT_RELU>(v[i]);
       break;
     case B2X_ACT_GELU:
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = act_fwd<B2X_ACT_GELU>(v[i]);
+      for (int i = 0; i < N; ++i) v[i] = act_fwd<B2X_ACT_GELU>(v[i]);
       break;
     case B2X_ACT_GELU_TANH:
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = act_fwd<B2X_ACT_GELU_TANH>(v[i]);
+      for (int i = 0; i < N; ++i) v[i] = act_fwd<B2X_ACT_GELU_TANH>(v[i]);
       break;
     case B2X_ACT_SILU:
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = act_fwd<B2X_ACT_SILU>(v[i]);
+      for (int i = 0; i < N; ++i) v[i] = act_fwd<B2X_ACT_SILU>(v[i]);
       break;
     default:
       break;

@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kTkThreads, 2)
     mbar_wait(done, 0, abort_flag, kStatusTimeoutEpilogue);
     __syncwarp();
     tc_fence_after();
-    float* part = reinterpret_cast<float*>(smem) + warp * 32 + lane;
+    const uint32_t part = smem_u32(smem) + (warp * 32 + lane) * 4;
 #pragma unroll
     for (int c0 = 0; c0 < NT; c0 += 16) {
       uint32_t v[16];
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kTkThreads, 2)
       tmem_ld_wait();
       tmem_regs_after_wait(v);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) part[(c0 + i) * kTkRows] = k1 > k0 ? __uint_as_float(v[i]) : 0.0f;
+      for (int i = 0; i < 16; ++i) st_shared_f32(part + (c0 + i) * kTkRows * 4, k1 > k0 ? __uint_as_float(v[i]) : 0.0f);
     }
     tc_fence_before();
   }
@@ -192,11 +192,11 @@ __global__ void __launch_bounds__(kTkThreads, 2)
   else
     __syncthreads();
   const uint32_t tile = smem_u32(smem);
-  auto fetch = [&](int m, int col) {
+  auto fetch4 = [&](int m, int col) {
     const uint32_t at = tile + (uint32_t)(m * kTkRows + col) * 4;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (p.splits == 1) {
-      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(s.x), "=f"(s.y), "=f"(s.z), "=f"(s.w) : "r"(at) : "memory");
+      s = ld_shared_f32x4(at);
     } else {
       for (int r = 0; r < p.splits; ++r) {
         float4 f;
@@ -213,13 +213,15 @@ __global__ void __launch_bounds__(kTkThreads, 2)
     const float hs = __ldg(p.h_scale);
     const float inv = hs == 0.0f ? 0.0f : __fdiv_rn(1.0f, hs);
     float amax = 0.0f;
-    tok_finish_swiglu(p, u.e, u.row0, u.nt * kTkRows, u.cnt, rank * kTkWarps + warp, p.splits * kTkWarps, lane, inv, amax, fetch);
+    tok_finish_swiglu(p, u.e, u.row0, u.nt * kTkRows, u.cnt, rank * kTkWarps + warp, p.splits * kTkWarps, lane, inv, amax, fetch4);
     if (p.h_amax) {
       const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
       if (lane == 0 && m) atomicMax(reinterpret_cast<unsigned*>(p.h_amax), m);
     }
   } else {
-    tok_finish(p, u.e, u.row0, u.nt * kTkRows, u.cnt, rank * kTkWarps + warp, p.splits * kTkWarps, lane, fetch);
+    const TokCols cols = tok_cols(p, u.e, u.nt * kTkRows, lane);
+    for (int m = rank * kTkWarps + warp; m < u.cnt; m += p.splits * kTkWarps)
+      tok_finish<1>(p, cols, u.row0 + m, 0, 1u, [&](int) { return fetch4(m, 4 * lane); });
   }
   __syncwarp();
   if (p.splits > 1)
@@ -239,12 +241,17 @@ __global__ void __launch_bounds__(kTkThreads, 2)
 // those rows and half of the tokens, 32 KB per CTA and K block where a single CTA's 128 x 256 tile needs 48 KB (no
 // multicast).  The tile is as wide as its tokens need, in steps of 32.  Two accumulators let the two epilogue
 // warpgroups of a CTA work behind the next tile's MMAs.  Roles as in fp8_gemm_pair.cu: warp 0 loads, warp 1 of the even
-// CTA issues the MMAs, warp 2 allocates TMEM, warps 4-11 finish tiles.  The units are found by every role itself: a warp
-// keeps 32 experts' ranges in its lanes (TokCursor) and moves on in the order of the units.
+// CTA issues the MMAs, warp 2 allocates TMEM, warps 4-11 finish tiles.
+//
+// Units have unequal widths, so they are handed out by cluster launch control: one cluster per unit is launched, a
+// running pair cancels clusters that have not started and takes their units.  Warp 3 of the even CTA asks, finds the
+// unit's expert (it keeps 32 experts' ranges in its lanes, TokCursor) and passes the unit to both CTAs through a ring of
+// four.  The other roles only read the ring: when each searched for its units itself, with the divisions and shuffles
+// that takes, the loads and MMAs stood still for some 4000 cycles at every change of unit.
 
 constexpr int kTpTokens = 256;    // tokens per unit
-constexpr int kTpBox = 64;        // tokens per load
-constexpr int kTpChunk = 16;      // tokens per epilogue step
+constexpr int kTpRing = 4;        // units handed out ahead
+constexpr int kTpReaders = 2 + 1 + 16;  // warps that read the ring: loads of both CTAs, MMA, epilogues of both
 constexpr int kTpBand = 16;       // token tiles whose X stays in L2 while the weight tiles go by
 
 template <int STAGES>
@@ -252,18 +259,19 @@ struct TpSmem {
   static constexpr int kWBytes = kTkRows * kBK;               // 16 KB
   static constexpr int kXBytes = (kTpTokens / 2) * kBK;       // 16 KB
   static constexpr int kStageBytes = kWBytes + kXBytes;
-  static constexpr int kCBytes = 2 * kTpChunk * kTkRows * 4;  // two steps of 8 KB per warpgroup
+  static constexpr int kCBytes = 2 * kTkChunk * kTkRows * 4;  // two steps of 8 KB per warpgroup
   static constexpr int kXOff = STAGES * kWBytes;
   static constexpr int kCOff = STAGES * kStageBytes;
   static constexpr int kBarOff = kCOff + 2 * kCBytes;
-  static constexpr int kAlloc = kBarOff + (2 * STAGES + 5) * 8 + 16 + 1024;
+  static constexpr int kRingOff = (kBarOff + (2 * STAGES + 5) * 8 + 8 + 15) / 16 * 16;  // answers, barriers, units
+  static constexpr int kAlloc = kRingOff + kTpRing * (2 * 16 + 3 * 8) + 1024;
 };
-constexpr int kTpStages = (kMaxDynSmem - 2 * TpSmem<1>::kCBytes - 1024 - 256) / TpSmem<1>::kStageBytes;
+constexpr int kTpStages = (kMaxDynSmem - 2 * TpSmem<1>::kCBytes - 1024 - 512) / TpSmem<1>::kStageBytes;
 
-// Walks the units in rising order; all lanes of a warp together.
+// Finds units, best in rising order; all lanes of a warp together.
 struct TokCursor {
-  int base, carry, total, s, mt;  // experts base .. base + 31; units before them, in them; lane's inclusive sum, token tiles
-  int64_t lo, rows;               // lane's range
+  int base, carry, total, s, mt, width;  // experts base .. base + 31; units before them, in them; lane's inclusive sum,
+  int64_t lo, rows;                      // token tiles and their width; lane's range
 };
 __device__ __forceinline__ void tok_chunk(const TokParams& p, TokCursor& c, int n2, int lane) {
   c.lo = c.rows = 0;
@@ -275,6 +283,7 @@ __device__ __forceinline__ void tok_chunk(const TokParams& p, TokCursor& c, int 
     c.rows = hi - c.lo;
   }
   c.mt = (int)((c.rows + kTpTokens - 1) / kTpTokens);
+  c.width = c.mt ? (int)((c.rows + c.mt - 1) / c.mt + 31) / 32 * 32 : 0;  // (mt - 1) * width < rows: width <= 256
   c.s = c.mt * n2;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -286,9 +295,13 @@ __device__ __forceinline__ void tok_chunk(const TokParams& p, TokCursor& c, int 
 // The unit, or cnt = 0 past the last one.  nt: index of the 256-row weight tile.
 __device__ __forceinline__ TokUnit tok_seek(const TokParams& p, TokCursor& c, int unit, int n2, int lane) {
   TokUnit u{0, 0, 0, 0};
+  if (unit < c.carry) {
+    c.base = c.carry = 0;
+    tok_chunk(p, c, n2, lane);
+  }
   while (unit >= c.carry + c.total) {
+    if (c.base + 32 >= p.E) return u;
     c.base += 32;
-    if (c.base >= p.E) return u;
     c.carry += c.total;
     tok_chunk(p, c, n2, lane);
   }
@@ -302,11 +315,11 @@ __device__ __forceinline__ TokUnit tok_seek(const TokParams& p, TokCursor& c, in
   const int m = band * kTpBand + r % width;
   u.e = c.base + src;
   u.nt = r / width;
-  u.row0 = lo + (int64_t)m * kTpTokens;
-  u.cnt = (int)min((int64_t)kTpTokens, rows - (int64_t)m * kTpTokens);
+  const int tokens = __shfl_sync(0xffffffffu, c.width, src);
+  u.row0 = lo + (int64_t)m * tokens;
+  u.cnt = (int)min((int64_t)tokens, rows - (int64_t)m * tokens);
   return u;
 }
-
 template <int W_KIND>
 __device__ __forceinline__ void tok_load_w_pair(const TokParams& p, void* dst, const CUtensorMap* m, uint32_t bar, int kb,
                                                 int e, int nt, uint64_t pol) {
@@ -321,7 +334,7 @@ __device__ __forceinline__ void tok_load_w_pair(const TokParams& p, void* dst, c
 template <int W_KIND>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_gemm_tokens_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                                const TokParams p) {
+                                const __grid_constant__ CUtensorMap tmXs, const TokParams p) {
   constexpr int STAGES = kTpStages;
   using L = TpSmem<STAGES>;
   static_assert(L::kAlloc <= kMaxDynSmem, "shared memory plan exceeds the opt-in limit");
@@ -334,11 +347,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* mma_done = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint8_t* answer = smem + L::kRingOff;
+  uint8_t* units = answer + kTpRing * 16;
+  uint64_t* answered = reinterpret_cast<uint64_t*>(units + kTpRing * 16);
+  uint64_t* ufull = answered + kTpRing;
+  uint64_t* uempty = ufull + kTpRing;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
 
   if (threadIdx.x == 0) {
+    for (int s = 0; s < kTpRing; ++s) {
+      mbar_init(&answered[s], 1);
+      mbar_init(&ufull[s], 1);
+      mbar_init(&uempty[s], kTpReaders);  // the even CTA's is used
+    }
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -354,6 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmW);
     tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmXs);
   }
   if (warp == 2) {
     tmem_alloc_pair(tmem_slot, 512);
@@ -363,10 +387,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int n2 = (p.n_tiles + 1) / 2;
-  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
-  TokCursor cur{0, 0, 0, 0, 0, 0, 0};
-  if (warp < 2 || warp >= kEpiWarp0) tok_chunk(p, cur, n2, lane);
+  // The next unit from the ring (`at` counts the reads); cnt = 0: none.  Whole warps.
+  auto next_unit = [&](int& at) {
+    const int s = at % kTpRing;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (mbar_wait_cluster(&ufull[s], (uint32_t)(at / kTpRing) & 1u, abort_flag, kStatusTimeoutProducer))
+      v = ld_shared_u32x4(smem_u32(units + s * 16));
+    __syncwarp();
+    if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&uempty[s]), 0));
+    ++at;
+    TokUnit u;
+    u.e = (int)v.x;
+    u.nt = (int)v.y;
+    u.row0 = (int)v.z;
+    u.cnt = (int)__shfl_sync(0xffffffffu, v.w, 0);  // one answer for the warp, even where a lane gave up
+    return u;
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------ loads (both CTAs)
@@ -374,12 +410,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     int stage = 0;
     uint32_t phase = 0, issued = 0, pend = 0;  // pend: bit s = phase of stage s's last load
     bool ok = true;
-    for (int unit = first; ok; unit += step) {
-      const TokUnit u = tok_seek(p, cur, unit, n2, lane);
+    int at = 0;
+    while (ok) {
+      const TokUnit u = next_unit(at);
       if (u.cnt == 0) break;
       if (lane == 0) {
         const int half = (u.cnt + 31) / 32 * 16;  // tokens per CTA
-        const int boxes = (half + kTpBox - 1) / kTpBox;
+        const CUtensorMap* mx = half > 64 ? &tmX : &tmXs;       // boxes of 128 or 64 tokens
+        const uint32_t bytes = 2 * (L::kWBytes + (half > 64 ? 128 : 64) * kBK);
         const int x0 = (int)u.row0 + (int)rank * half;
         for (int kb = 0; kb < p.k_tiles; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, kStatusTimeoutProducer)) {
@@ -387,11 +425,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);
-          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * (L::kWBytes + boxes * kTpBox * kBK));
-          uint8_t* sx = smem + L::kXOff + stage * L::kXBytes;
+          if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
           tok_load_w_pair<W_KIND>(p, smem + stage * L::kWBytes, &tmW, bar, kb, u.e, 2 * u.nt + (int)rank, pol_w);
-          for (int b = 0; b < boxes; ++b)
-            tma_load_2d_pair(sx + b * kTpBox * kBK, &tmX, bar, kb * kBK, x0 + b * kTpBox, pol_x);
+          tma_load_2d_pair(smem + L::kXOff + stage * L::kXBytes, mx, bar, kb * kBK, x0, pol_x);
           issued |= 1u << stage;
           pend = (pend & ~(1u << stage)) | (phase << stage);
           if (++stage == STAGES) stage = 0, phase ^= 1;
@@ -409,11 +445,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMAs (even CTA)
     if (leader) {
-      int stage = 0, local = 0;
+      const uint64_t desc_w = smem_desc_sw128(smem_u32(smem), W_KIND == 1 ? 128 * kBK : 16, 1024);
+      const uint64_t desc_x = smem_desc_sw128(smem_u32(smem + L::kXOff), 16, 1024);
+      int stage = 0, at = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int unit = first; ok; unit += step, ++local) {
-        const TokUnit u = tok_seek(p, cur, unit, n2, lane);
+      for (int local = 0; ok; ++local) {
+        const TokUnit u = next_unit(at);
         if (u.cnt == 0) break;
         if (lane == 0) {
           const int buf = local & 1;
@@ -427,13 +465,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               break;
             }
             tc_fence_after();
-            const uint32_t w = smem_u32(smem + stage * L::kWBytes), x = smem_u32(smem + L::kXOff + stage * L::kXBytes);
+            // the address fields of both descriptors move by constants: one addition each per MMA
+            const uint64_t w = desc_w + (uint32_t)stage * (L::kWBytes >> 4), x = desc_x + (uint32_t)stage * (L::kXBytes >> 4);
+            mma_f8f6f4_pair(d, w, x, idesc, kb > 0 ? 1u : 0u);
 #pragma unroll
-            for (int k = 0; k < kBK / 32; ++k)
-              mma_f8f6f4_pair(d,
-                              W_KIND == 1 ? smem_desc_sw128(w + k * 32 * 128, 128 * kBK, 1024)
-                                          : smem_desc_sw128(w + k * 32, 16, 1024),
-                              smem_desc_sw128(x + k * 32, 16, 1024), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+            for (int k = 1; k < kBK / 32; ++k)
+              mma_f8f6f4_pair(d, w + k * ((W_KIND == 1 ? 32 * 128 : 32) >> 4), x + k * (32 >> 4), idesc, 1u);
             mma_commit_pair_mc(&empty[stage], 0x3);
             if (++stage == STAGES) stage = 0, phase ^= 1;
           }
@@ -447,51 +484,143 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(mma_done, 0, &no_abort, kStatusTimeoutMma);
       }
     }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------ units (even CTA)
+    if (leader) {
+      const int n2 = (p.n_tiles + 1) / 2;
+      TokCursor cur{0, 0, 0, 0, 0, 0, 0, 0};
+      tok_chunk(p, cur, n2, lane);
+      int put = 0;
+      for (int unit = blockIdx.x >> 1, asked = 0;; ++asked) {
+        const int r = asked % kTpRing;
+        if (lane == 0 && unit >= 0) {  // ask for the one after it, then pass this one on
+          fence_proxy_async_smem();
+          mbar_arrive_expect_tx(&answered[r], 16);
+          clc_try_cancel(answer + r * 16, &answered[r]);
+        }
+        const TokUnit u = unit >= 0 ? tok_seek(p, cur, unit, n2, lane) : TokUnit{0, 0, 0, 0};
+        int next = -1;
+        if (lane == 0) {
+          if (u.cnt > 0 || unit < 0) {  // clusters past the last unit are only taken out of the way
+            const int s = put % kTpRing;
+            if (mbar_wait_cluster(&uempty[s], ((uint32_t)(put / kTpRing) & 1u) ^ 1u, abort_flag, kStatusTimeoutProducer))
+              for (uint32_t c = 0; c < 2; ++c) {
+                st_cluster_v4(mapa_shared(smem_u32(units + s * 16), c), make_int4(u.e, u.nt, (int)u.row0, u.cnt));
+                mbar_arrive_cluster(mapa_shared(smem_u32(&ufull[s]), c));
+              }
+            ++put;
+          }
+          if (unit >= 0) {
+            volatile int no_abort = 0;
+            if (mbar_wait(&answered[r], (uint32_t)(asked / kTpRing) & 1u, &no_abort, kStatusTimeoutProducer)) {
+              const int cta = clc_first_ctaid_x(answer + r * 16);
+              next = cta < 0 ? -1 : cta >> 1;
+            }
+          }
+        }
+        if (unit < 0) break;
+        unit = __shfl_sync(0xffffffffu, next, 0);
+      }
+    }
   } else if (warp >= kEpiWarp0) {
     // ------------------------------------------------------------ epilogue (both CTAs)
     const int e = (warp - kEpiWarp0) >> 2, q = warp & 3;
     const uint32_t bar_id = 1 + e;
     const int wg_tid = threadIdx.x - (kEpiWarp0 + 4 * e) * 32;
-    float* stage_c = reinterpret_cast<float*>(smem + L::kCOff + e * L::kCBytes);
+    const uint32_t stage_c = smem_u32(smem + L::kCOff + e * L::kCBytes);
     const uint32_t tempty_leader = mapa_shared(smem_u32(&tempty[e]), 0);
     float inv = 0.0f, amax = 0.0f;
     if constexpr (W_KIND == 2) {
       const float hs = __ldg(p.h_scale);
       inv = hs == 0.0f ? 0.0f : __fdiv_rn(1.0f, hs);
     }
-    int local = 0;
-    for (int unit = first;; unit += step, ++local) {
-      const TokUnit u = tok_seek(p, cur, unit, n2, lane);
+    int at = 0;
+    for (int local = 0;; ++local) {
+      const TokUnit u = next_unit(at);
       if (u.cnt == 0) break;
       if ((local & 1) != e) continue;
-      const bool ok = mbar_wait(&tfull[e], (local >> 1) & 1, abort_flag, kStatusTimeoutEpilogue);
-      if (!wg_all(ok, bar_id)) break;
-      tc_fence_after();
       const uint32_t t_row = tmem_base + e * kTpTokens + ((uint32_t)(q * 32) << 16);
       const int n0 = (2 * u.nt + (int)rank) * kTkRows;
-      const int chunks = (u.cnt + kTpChunk - 1) / kTpChunk;
+      const int chunks = (u.cnt + kTkChunk - 1) / kTkChunk;
+      auto release = [&]() {  // all 128 threads have read the accumulator
+        if (wg_tid == 0) mbar_arrive_cluster_relaxed(tempty_leader);
+      };
+      auto ready = [&]() {
+        const bool ok = mbar_wait(&tfull[e], (local >> 1) & 1, abort_flag, kStatusTimeoutEpilogue);
+        const bool all = wg_all(ok, bar_id);
+        tc_fence_after();
+        return all;
+      };
+      if constexpr (W_KIND == 2) {
+        // Lanes 0-15 hold gate rows, lanes 16-31 the up rows of the same 16 columns of h.  Of two neighbouring tokens a
+        // gate lane hands the second's value over and an up lane the first's: each then has gate and up of one token.
+        // The tile's codes, [256 tokens][64 bytes], fill the staging; one barrier, then whole 64-byte rows leave.
+        const float sw = tok_scale_w(p, u.e);
+        const float fmax = p.h_e5m2 ? 57344.0f : 448.0f;
+        const int odd = lane >> 4;
+        if (!ready()) break;
 #pragma unroll 1
-      for (int c = 0; c < chunks; ++c) {
-        uint32_t v[kTpChunk];
-        tmem_ld_32x32b_x16(t_row + c * kTpChunk, v);
-        tmem_ld_wait();
-        tmem_regs_after_wait(v);
-        float* buf = stage_c + (c & 1) * kTpChunk * kTkRows;
+        for (int c = 0; c < chunks; ++c) {
+          uint32_t v[kTkChunk];
+          tmem_ld_32x32b_x16(t_row + c * kTkChunk, v);
+          // lane l: the factor of token l of the step
+          const int m0 = min(c * kTkChunk + (lane & 15), u.cnt - 1);
+          const float alpha = tok_alpha(p, u.row0 + m0, sw);
+          tmem_ld_wait();
+          tmem_regs_after_wait(v);
 #pragma unroll
-        for (int i = 0; i < kTpChunk; ++i) buf[i * kTkRows + q * 32 + lane] = __uint_as_float(v[i]);
+          for (int i = 0; i < kTkChunk / 2; ++i) {
+            const float a = __uint_as_float(v[2 * i]), b = __uint_as_float(v[2 * i + 1]);
+            const float other = __shfl_xor_sync(0xffffffffu, odd ? a : b, 16);
+            const float h = tok_swiglu(odd ? other : a, odd ? b : other, __shfl_sync(0xffffffffu, alpha, 2 * i + odd));
+            const int m = c * kTkChunk + 2 * i + odd;
+            if (m < u.cnt) amax = fmaxf(amax, fabsf(h));
+            const float y = swiglu_clamp(__fmul_rn(h, inv), fmax);
+            st_shared_u8(stage_c + m * 64 + q * 16 + (lane & 15), p.h_e5m2 ? cvt_e5m2x2(y, 0.0f) : cvt_e4m3x2(y, 0.0f));
+          }
+        }
         tc_fence_before();
-        // the other half of the staging was read before the barrier of the step before: one barrier a step
         named_bar_sync(bar_id, 128);
-        if (c + 1 == chunks && wg_tid == 0) mbar_arrive_cluster_relaxed(tempty_leader);
-        auto fetch = [&](int m, int col) { return *reinterpret_cast<const float4*>(buf + m * kTkRows + col); };
-        const int cnt = min(kTpChunk, u.cnt - c * kTpChunk);
-        const int64_t row0 = u.row0 + c * kTpChunk;
-        if constexpr (W_KIND == 2)
-          tok_finish_swiglu(p, u.e, row0, n0, cnt, q, 4, lane, inv, amax, fetch);
-        else
-          tok_finish(p, u.e, row0, n0, cnt, q, 4, lane, fetch);
+        release();
+        for (int i = wg_tid; i < u.cnt * 4; i += 128)
+          __stcs(reinterpret_cast<uint4*>(p.h + (u.row0 + (i >> 2)) * p.ld_h + n0 / 2 + (i & 3) * 16),
+                 ld_shared_u32x4(stage_c + i * 16));
+      } else {
+        const TokCols cols = tok_cols(p, u.e, n0, lane);
+        const bool fast = n0 + kTkRows <= p.N && p.vec_out && (!p.residual || p.vec_res) && (!p.pre || p.vec_pre);
+        const int kind = !fast ? 16 : (p.half ? 8 : 0) + (p.act ? 4 : 0) + (p.residual ? 2 : 0) + (p.pre ? 1 : 0);
+        if (!ready()) break;
+        switch (kind) {
+#define B2X_TILE(H, A, R, P)                                                                                              \
+  case 8 * H + 4 * A + 2 * R + P:                                                                                         \
+    tok_tile<H, A, R, P>(p, cols, t_row, u.row0, u.cnt, q, lane, stage_c, bar_id, release);                               \
+    break;
+          B2X_TILE(0, 0, 0, 0) B2X_TILE(0, 0, 0, 1) B2X_TILE(0, 0, 1, 0) B2X_TILE(0, 0, 1, 1)
+          B2X_TILE(0, 1, 0, 0) B2X_TILE(0, 1, 0, 1) B2X_TILE(0, 1, 1, 0) B2X_TILE(0, 1, 1, 1)
+          B2X_TILE(1, 0, 0, 0) B2X_TILE(1, 0, 0, 1) B2X_TILE(1, 0, 1, 0) B2X_TILE(1, 0, 1, 1)
+          B2X_TILE(1, 1, 0, 0) B2X_TILE(1, 1, 0, 1) B2X_TILE(1, 1, 1, 0) B2X_TILE(1, 1, 1, 1)
+#undef B2X_TILE
+          default:  // the last columns, or rows off the 8-byte grid: one step at a time, every access checked
+#pragma unroll 1
+            for (int c = 0; c < chunks; ++c) {
+              uint32_t v[kTkChunk];
+              tmem_ld_32x32b_x16(t_row + c * kTkChunk, v);
+              tmem_ld_wait();
+              tmem_regs_after_wait(v);
+              const uint32_t buf = stage_c + (c & 1) * kTkChunk * kTkRows * 4;
+#pragma unroll
+              for (int i = 0; i < kTkChunk; ++i) st_shared_f32(buf + (i * kTkRows + q * 32 + lane) * 4, __uint_as_float(v[i]));
+              tc_fence_before();
+              named_bar_sync(bar_id, 128);
+              if (c + 1 == chunks) release();
+              const int left = u.cnt - c * kTkChunk - q;
+              const uint32_t live = (left > 0 ? 1u : 0u) | (left > 4 ? 2u : 0u) | (left > 8 ? 4u : 0u) | (left > 12 ? 8u : 0u);
+              tok_finish<4>(p, cols, u.row0 + c * kTkChunk + q, 4, live,
+                            [&](int i) { return ld_shared_f32x4(buf + ((q + 4 * i) * kTkRows + 4 * lane) * 4); });
+            }
+        }
       }
-      named_bar_sync(bar_id, 128);  // the next tile's first step writes the staging again
+      named_bar_sync(bar_id, 128);  // the next tile writes the staging again
     }
     if constexpr (W_KIND == 2) {
       if (p.h_amax) {
@@ -549,7 +678,7 @@ static cudaError_t launch_tokens_nt(const TokLaunch& g, const CUtensorMap& tmX, 
 }
 
 template <int W_KIND>
-static cudaError_t launch_tokens_pair_t(const TokLaunch& g, const CUtensorMap& tmX, int64_t units, cudaStream_t st) {
+static cudaError_t launch_tokens_pair_t(const TokLaunch& g, const CUtensorMap (&tmX)[2], int64_t units, cudaStream_t st) {
   using L = TpSmem<kTpStages>;
   auto kern = fp8_gemm_tokens_pair_kernel<W_KIND>;
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), L::kAlloc);
@@ -565,9 +694,8 @@ static cudaError_t launch_tokens_pair_t(const TokLaunch& g, const CUtensorMap& t
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const int64_t pairs = std::min<int64_t>(units, g.num_sms / 2);
-  cfg.gridDim = dim3((unsigned)(2 * std::max<int64_t>(pairs, 1)), 1, 1);
-  e = cudaLaunchKernelEx(&cfg, kern, g.tmW, tmX, g.p);
+  cfg.gridDim = dim3((unsigned)(2 * units), 1, 1);  // one cluster per unit
+  e = cudaLaunchKernelEx(&cfg, kern, g.tmW, tmX[0], tmX[1], g.p);
   note_launch(1);
   return e;
 }
@@ -580,22 +708,27 @@ static b2x_status launch_tokens(TokLaunch& g, const char* who, cudaStream_t st) 
   const bool moe = p.offsets != nullptr;
   const double active = moe ? expected_active(p.rows, p.E) : 1.0;
   const double mean = (double)p.rows / active;
+  // Pairs or single CTAs.  Up to 32 tokens per product the weights are all there is to read, and the short single-CTA
+  // tiles do that best (64 experts x 7168 x 2048, 40 rows: 80 us against 91 us on pairs; 2048 rows: 181 and 179).  Above,
+  // pairs win where their units fill the GPU: twice up to 96 tokens (8 experts x 4096 x 4096, 512 rows, 128 units: 30.5
+  // and 34.5; 32 experts x 4096 x 7168, 2048 rows, 512 units: 184 and 165), half of it for wider tiles, whose work per
+  // byte is twice that of the single CTAs' (256 x 8192 x 8192, 32 units: 25.9 and 29.7; 384 rows, 64 units: 47.6 and 31.9).
+  const int pairs = g.num_sms / 2;
   const double mean256 = ceil(mean / kTpTokens);
   const double units2 = std::max(1.0, moe ? active * mean256 : mean256) * ((p.n_tiles + 1) / 2);
-  bool pair = units2 >= g.num_sms / 2;
-#ifdef B2X_TOK_FORCE
-  if (const char* f = getenv("B2X_TOK")) pair = f[0] == '2';
-#endif
+  const bool pair = mean > 96 ? units2 >= pairs / 2 : (mean > 32 && units2 >= 2 * pairs);
   if (pair) {
     const int64_t most = (moe ? p.rows / kTpTokens + std::min<int64_t>(p.E, p.rows) : (p.rows + kTpTokens - 1) / kTpTokens) *
                          ((p.n_tiles + 1) / 2);
-    if (most >= (1LL << 31)) return fail(B2X_ERR_UNSUPPORTED, "%s: too many tiles", who);
+    if (2 * most >= (1LL << 31)) return fail(B2X_ERR_UNSUPPORTED, "%s: too many tiles", who);
     p.idesc = idesc_f8f6f4(g.w_fmt, g.x_fmt, g.w_kind == 1 ? 1 : 0, 0, 2 * kTkRows, 0);
     p.l2_w = 0;
-    CUtensorMap tmX;
-    b2x_status s = encode_2d(&tmX, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.x, (uint64_t)p.K, (uint64_t)p.rows, (uint64_t)g.ld_x,
-                             128, kTpBox, CU_TENSOR_MAP_SWIZZLE_128B, "x");
-    if (s != B2X_OK) return s;
+    CUtensorMap tmX[2];
+    for (int i = 0; i < 2; ++i) {
+      b2x_status s = encode_2d(&tmX[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, g.x, (uint64_t)p.K, (uint64_t)p.rows,
+                               (uint64_t)g.ld_x, 128, i ? 64 : 128, CU_TENSOR_MAP_SWIZZLE_128B, "x");
+      if (s != B2X_OK) return s;
+    }
     cudaError_t e = g.w_kind == 0   ? launch_tokens_pair_t<0>(g, tmX, most, st)
                     : g.w_kind == 1 ? launch_tokens_pair_t<1>(g, tmX, most, st)
                                     : launch_tokens_pair_t<2>(g, tmX, most, st);
@@ -610,14 +743,16 @@ static b2x_status launch_tokens(TokLaunch& g, const char* who, cudaStream_t st) 
   const int64_t tok_tiles = moe ? p.rows / nt + std::min<int64_t>(p.E, p.rows) : (p.rows + nt - 1) / nt;
   const int64_t units = tok_tiles * p.n_tiles;
   const double planned = std::max(1.0, moe ? active * ceil(mean / nt) : (double)tok_tiles) * p.n_tiles;
-  // K ranges: as many as fill the SMs' two slots best, a little preference for fewer.
-  double best = -1;
-  for (int s = 1; s <= 8; s *= 2) {
-    const int per = (p.k_tiles + s - 1) / s;
-    if (s > 1 && (per < 4 || (int64_t)(s - 1) * per >= p.k_tiles)) break;
-    const double ctas = planned * s, slots = 2.0 * g.num_sms;
-    const double eff = ctas / (ceil(ctas / slots) * slots) * pow(0.97, log2((double)s));
-    if (eff > best) best = eff, p.splits = s;
+  // K ranges: none if the tiles reach every SM, else the fewest that do, but 8 only where 4 would leave more than half
+  // of the SMs idle: a larger cluster costs more to place and to add up (1 x 28672 x 8192, 224 tiles: 42 us with one
+  // range, 44, 52 and 60 with 2, 4 and 8; 1 x 8192 x 8192, 64 tiles: 23, 14.5, 11.2, 16; 1 x 1024 x 16384, 8 tiles: 41, 23,
+  // 13.8, 9.5).
+  p.splits = 1;
+  while (p.splits < 8 && planned * p.splits < g.num_sms) {
+    const int s = 2 * p.splits, per = (p.k_tiles + s - 1) / s;
+    if (per < 4 || (int64_t)(s - 1) * per >= p.k_tiles) break;  // short ranges, or an empty one
+    if (s == 8 && planned * 4 >= 64) break;
+    p.splits = s;
   }
   if (units * p.splits >= (1LL << 31)) return fail(B2X_ERR_UNSUPPORTED, "%s: too many tiles", who);
   p.idesc = idesc_f8f6f4(g.w_fmt, g.x_fmt, g.w_kind == 1 ? 1 : 0, 0, kTkRows, 0);
@@ -659,6 +794,7 @@ static b2x_status encode_weights(CUtensorMap* m, int kind, const void* w, int64_
   return B2X_OK;
 }
 
+// Rows of 16-bit values that start on 8-byte boundaries.
 static bool even_rows(const void* p, int64_t ld) { return ((uintptr_t)p % 8) == 0 && ld % 4 == 0; }
 
 static int b2x_device_sms(const char* who, b2x_status& s) {
