@@ -33,6 +33,11 @@ class MoePlan(NamedTuple):
     rows: torch.Tensor     # int32 [tokens, top_k]
 
 
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
+_byref = ctypes.byref
+
+
 def _device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
     """The one CUDA device of all tensors."""
     if not first.is_cuda:
@@ -46,11 +51,12 @@ def _device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.devic
 
 def _call(dev: torch.device, fn, *args) -> None:
     """fn(*args, stream) with `dev` current and its current stream."""
-    if dev.index == torch._C._cuda_getDevice():
-        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    i = dev.index
+    if i == _current_device():
+        st = fn(*args, _current_stream(i))
     else:
         with torch.cuda.device(dev):
-            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+            st = fn(*args, _current_stream(i))
     if st:
         L.check(st)
 
@@ -63,22 +69,26 @@ def _matrix(t: torch.Tensor, what: str) -> torch.Tensor:
 
 def _ld(t: torch.Tensor) -> int:
     """Row stride in elements; a single row (or column) may have any."""
-    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+    rows, cols = t.shape
+    return max(t.stride(0), cols) if rows <= 1 else t.stride(0)
 
 
 def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
     """A 2-D tensor with unit column stride and rows that do not overlap."""
+    if t.dim() == 2 and t.is_contiguous():
+        return t
     t = _matrix(t, what)
     return t if t.shape[0] <= 1 or t.stride(0) >= t.shape[1] else t.contiguous()
 
 
-def _output(out: Optional[torch.Tensor], shape, dtype, dev, what: str, pad: int = 8) -> torch.Tensor:
-    """`out` checked, or a new tensor whose row pitch is a multiple of `pad` elements."""
+def _output(out: Optional[torch.Tensor], shape, dtype, like: torch.Tensor, what: str, pad: int = 8) -> torch.Tensor:
+    """`out` checked, or a new tensor on like's device whose row pitch is a multiple of `pad` elements."""
+    dev = like.device
     if out is None:
         n = shape[1]
-        p = -(-n // pad) * pad
-        t = torch.empty((shape[0], p), dtype=dtype, device=dev)
-        return t if p == n else t[:, :n]
+        if n % pad == 0:
+            return like.new_empty(shape, dtype=dtype)
+        return like.new_empty((shape[0], -(-n // pad) * pad), dtype=dtype)[:, :n]
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != dev:
         raise ValueError(f"{what} must be a {dtype} tensor of shape {tuple(shape)} on {dev}")
     if (out.stride(1) != 1 and out.shape[1] > 1) or (out.shape[0] > 1 and out.stride(0) < out.shape[1]):
@@ -92,14 +102,15 @@ def _scale(t: Optional[torch.Tensor], what: str, *counts: int) -> Optional[torch
         return None
     if t.numel() not in counts:
         raise ValueError(f"{what} must have {' or '.join(str(c) for c in dict.fromkeys(counts))} elements, got {t.numel()}")
-    t = t.reshape(-1)
-    return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
+    if t.dtype is torch.float32 and t.is_contiguous():
+        return t
+    return t.reshape(-1).to(torch.float32).contiguous()
 
 
 def _ints(t: torch.Tensor, what: str) -> torch.Tensor:
     if t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
 # ----------------------------------------------------------------------------
@@ -141,14 +152,15 @@ def gemm_epilogue(a: torch.Tensor, b: torch.Tensor, *, scale_a: Optional[torch.T
             raise TypeError(f"residual must be {out_dtype} like the output, got {residual.dtype}")
         residual = _rows(residual, "residual")
     sa, sb = _scale(scale_a, "scale_a", 1), _scale(scale_b, "scale_b", 1)
-    c = _output(None, (M, N), out_dtype, dev, "out")
-    pre = _output(None, (M, N), out_dtype, dev, "pre") if return_pre else None
+    c = _output(None, (M, N), out_dtype, a, "out")
+    pre = _output(None, (M, N), out_dtype, a, "pre") if return_pre else None
     if M and N:
         if K == 0:
             raise ValueError("gemm_epilogue needs K > 0")
         if M > 1 and a.stride(0) < K:  # rows that overlap
             a = a.contiguous()
-        if min(b.stride()) != 1 or max(b.stride()) < (K if b.stride(0) == 1 else N):
+        sk, sn = b.stride()
+        if min(sk, sn) != 1 or max(sk, sn) < (K if sk == 1 else N):
             b = b.contiguous()
         a, b = _tma_friendly(a, b)
         K = a.shape[1]
@@ -172,7 +184,7 @@ def gemm_epilogue(a: torch.Tensor, b: torch.Tensor, *, scale_a: Optional[torch.T
             ep.residual, ep.ld_residual = residual.data_ptr(), _ld(residual)
         if pre is not None:
             ep.pre, ep.ld_pre = pre.data_ptr(), _ld(pre)
-        _call(dev, L.lib().b2x_fp8_gemm_epilogue, ctypes.byref(g), ctypes.byref(ep))
+        _call(dev, L.lib().b2x_fp8_gemm_epilogue, _byref(g), _byref(ep))
     return (c, pre) if return_pre else c
 
 
@@ -189,8 +201,8 @@ def epilogue_backward(grad: torch.Tensor, pre: torch.Tensor, activation: Optiona
         raise TypeError(f"grad and pre must both be float32, bfloat16 or float16, got {grad.dtype} and {pre.dtype}")
     M, N = grad.shape
     grad, pre = _rows(grad, "grad"), _rows(pre, "pre")
-    out = _output(None, (M, N), grad.dtype, dev, "d_pre")
-    db = torch.empty(N, dtype=torch.float32, device=dev) if bias_grad else None
+    out = _output(None, (M, N), grad.dtype, grad, "d_pre")
+    db = grad.new_empty(N, dtype=torch.float32) if bias_grad else None
     _call(dev, L.lib().b2x_epilogue_backward, grad.data_ptr(), _ld(grad), pre.data_ptr(), _ld(pre), out.data_ptr(), _ld(out),
           db.data_ptr() if db is not None else None, FLOAT_DTYPES[grad.dtype], M, N, ACTIVATIONS[activation])
     return out, db
@@ -235,12 +247,12 @@ def moe_route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias:
     a = _route_args(logits, top_k, score, renormalize, scale)
     a.num_groups, a.top_groups, a.group_top2 = num_groups, top_groups, group_score == "top2"
     k = max(top_k, 0)
-    weights = torch.empty((T, k), dtype=torch.float32, device=dev)
-    experts = torch.empty((T, k), dtype=torch.int32, device=dev)
+    weights = logits.new_empty((T, k), dtype=torch.float32)
+    experts = logits.new_empty((T, k), dtype=torch.int32)
     if bias is not None:
         a.bias = bias.data_ptr()
     a.weights, a.indices = weights.data_ptr(), experts.data_ptr()
-    _call(dev, L.lib().b2x_moe_route, ctypes.byref(a))
+    _call(dev, L.lib().b2x_moe_route, _byref(a))
     return weights, experts
 
 
@@ -257,10 +269,10 @@ def moe_route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, experts
         raise ValueError(f"experts {tuple(experts.shape)} and grad_weights {tuple(grad_weights.shape)} must be [{T}, top_k]")
     experts = _ints(experts, "experts")
     d = grad_weights if grad_weights.dtype == torch.float32 and grad_weights.is_contiguous() else grad_weights.to(torch.float32).contiguous()
-    out = torch.empty((T, E), dtype=logits.dtype, device=dev)
+    out = logits.new_empty((T, E))
     a = _route_args(logits, experts.shape[1], score, renormalize, scale)
     a.indices = experts.data_ptr()
-    _call(dev, L.lib().b2x_moe_route_backward, ctypes.byref(a), d.data_ptr(), out.data_ptr(), E)
+    _call(dev, L.lib().b2x_moe_route_backward, _byref(a), d.data_ptr(), out.data_ptr(), E)
     return out
 
 
@@ -288,10 +300,10 @@ def moe_dispatch(x: torch.Tensor, experts: torch.Tensor, num_experts: int, *, dt
     experts = _ints(experts, "experts")
     k = experts.shape[1]
     given = _scale(scale, "scale", 1)
-    q = _output(out, (T * k, H), dtype, dev, "out", 16)
-    scales = torch.empty(T * k, dtype=torch.float32, device=dev) if given is None else given
-    offsets = torch.empty(max(num_experts, 0) + 1, dtype=torch.int32, device=dev)
-    rows = torch.empty((T, k), dtype=torch.int32, device=dev)
+    q = _output(out, (T * k, H), dtype, x, "out", 16)
+    scales = x.new_empty(T * k, dtype=torch.float32) if given is None else given
+    offsets = x.new_empty(max(num_experts, 0) + 1, dtype=torch.int32)
+    rows = x.new_empty((T, k), dtype=torch.int32)
     a = L.MoeDispatchArgs()
     a.x, a.x_type, a.tokens, a.cols, a.ld_x = x.data_ptr(), IN_DTYPES[x.dtype], T, H, _ld(x)
     a.indices, a.top_k, a.experts = experts.data_ptr(), k, num_experts
@@ -301,7 +313,7 @@ def moe_dispatch(x: torch.Tensor, experts: torch.Tensor, num_experts: int, *, dt
     else:
         a.given = given.data_ptr()
     a.offsets, a.rows = offsets.data_ptr(), rows.data_ptr()
-    _call(dev, L.lib().b2x_moe_dispatch, ctypes.byref(a))
+    _call(dev, L.lib().b2x_moe_dispatch, _byref(a))
     return q, scales, MoePlan(offsets, rows)
 
 
@@ -331,7 +343,7 @@ def moe_combine(y: torch.Tensor, rows: torch.Tensor, weights: Optional[torch.Ten
         if tuple(residual.shape) != (T, H) or residual.dtype != y.dtype:
             raise ValueError(f"residual must be a {y.dtype} tensor of shape {(T, H)}")
         residual = _rows(residual, "residual")
-    out = _output(None, (T, H), y.dtype, dev, "out")
+    out = _output(None, (T, H), y.dtype, y, "out")
     _call(dev, L.lib().b2x_moe_combine, y.data_ptr(), R, _ld(y), rows.data_ptr(), weights.data_ptr() if weights is not None else None,
           T, k, H, residual.data_ptr() if residual is not None else None, _ld(residual) if residual is not None else 0,
           out.data_ptr(), _ld(out), FLOAT_DTYPES[y.dtype])
@@ -351,8 +363,8 @@ def moe_combine_backward(grad: torch.Tensor, y: torch.Tensor, rows: torch.Tensor
     R, H = y.shape
     if tuple(grad.shape) != (T, H):
         raise ValueError(f"grad must have shape {(T, H)}, got {tuple(grad.shape)}")
-    dy = _output(out, (R, H), y.dtype, dev, "out")
-    dw = torch.empty((T, k), dtype=torch.float32, device=dev)
+    dy = _output(out, (R, H), y.dtype, y, "out")
+    dw = y.new_empty((T, k), dtype=torch.float32)
     _call(dev, L.lib().b2x_moe_combine_backward, grad.data_ptr(), _ld(grad), y.data_ptr(), R, _ld(y), rows.data_ptr(),
           weights.data_ptr(), T, k, H, dy.data_ptr(), _ld(dy), dw.data_ptr(), FLOAT_DTYPES[y.dtype])
     return dy, dw
@@ -417,9 +429,9 @@ def moe_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, scale_x
     if out_dtype not in OUT_DTYPES:
         raise TypeError(f"moe_gemm output must be bfloat16 or float16, got {out_dtype}")
     a, keep = _moe_gemm_args(x, w, offsets, scale_x, scale_w, "moe_gemm", False)
-    y = _output(out, (a.rows, a.N), out_dtype, dev, "out")
+    y = _output(out, (a.rows, a.N), out_dtype, x, "out")
     if a.rows and a.N:
-        _call(dev, L.lib().b2x_moe_gemm, ctypes.byref(a), y.data_ptr(), OUT_DTYPES[out_dtype], _ld(y))
+        _call(dev, L.lib().b2x_moe_gemm, _byref(a), y.data_ptr(), OUT_DTYPES[out_dtype], _ld(y))
     return y
 
 
@@ -442,8 +454,8 @@ def moe_gemm_swiglu(x: torch.Tensor, w_gu: torch.Tensor, offsets: torch.Tensor, 
         w_gu = w_gu.contiguous()
     a, keep = _moe_gemm_args(x, w_gu, offsets, scale_x, scale_w, "moe_gemm_swiglu", True)
     hs = _scale(h_scale, "h_scale", 1)
-    h = _output(out, (a.rows, a.N // 2), h_dtype, dev, "out", 16)
+    h = _output(out, (a.rows, a.N // 2), h_dtype, x, "out", 16)
     if a.rows and a.N:
-        _call(dev, L.lib().b2x_moe_gemm_swiglu, ctypes.byref(a), h.data_ptr(), FP8_DTYPES[h_dtype], _ld(h), hs.data_ptr(),
+        _call(dev, L.lib().b2x_moe_gemm_swiglu, _byref(a), h.data_ptr(), FP8_DTYPES[h_dtype], _ld(h), hs.data_ptr(),
               h_amax.data_ptr() if h_amax is not None else None)
     return h

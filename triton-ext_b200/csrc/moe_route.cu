@@ -1,9 +1,13 @@
 // Expert routing for sm_100a: scores, balance bias, groups, top-k and renormalised weights of a mixture of experts, and
 // the gradient of the weights.
 //
-// One warp owns a token; lane l holds the logits of experts 32 i + l in registers, so a row is read once, coalesced.
-// The k choices are taken one after the other: a warp-wide maximum of order-preserving 32-bit keys (redux.sync), then the
-// lowest index that has it.
+// One warp owns a token; lane l holds the logits of experts VPL l .. VPL l + VPL - 1 in registers, so a row is read once
+// and a group of experts is a run of lanes.  Bound: HBM for many tokens (tokens * experts logits in), latency for few; in
+// between the instructions of the selection, so that takes few.  Choices become order-preserving 32-bit keys.  The
+// (k + 1)-th largest of the 32 lanes' maxima (redux.sync) is a bound that at least k + 1 keys reach and few more; those
+// (almost always at most 32) are packed one to a lane in the order of their index, and each counts the better ones.  Where
+// more than 32 reach the bound the choices are taken one after the other instead.  What bounds the kernel is the integer
+// pipe, at half rate: comparisons and selections.
 //
 // What is compared.  Without a bias s is monotone in the logit, so the logits themselves are the keys and the choice is
 // exact.  With a bias (and for sums of two) the keys are fp32 values of s + b, each off by at most
@@ -29,6 +33,8 @@ struct RouteParams {
   int64_t tokens;
   int type, E, k;
   int sigmoid, renorm, groups, top_groups, top2;
+  int lanes_per_group;  // where a group is a run of 2^n whole lanes, else 0
+  int vec;              // rows allow 4-value loads
   float scale;
   const float* bias;
   float* weights;
@@ -37,6 +43,7 @@ struct RouteParams {
   const float* d_weights;
   void* d_logits;
   int64_t ld_d;
+  int vec_d;
 };
 
 // Unsigned order of floats: masked (-inf) 0, then rising, NaN on top; -0 and +0 are one value.
@@ -75,9 +82,46 @@ __device__ __forceinline__ void warp_argmax(double& v, int& at) {
   }
 }
 
+// VPL consecutive logits of a row as fp32; past the last expert -inf.
+template <int VPL>
+__device__ __forceinline__ void load_logits(const RouteParams& p, int64_t row, int lane, float (&l)[VPL]) {
+  const int e0 = lane * VPL;
+  const int bytes = p.type == B2X_F32 ? 4 : 2;
+  if (VPL % 4 == 0 && p.vec && e0 + VPL <= p.E) {
+    const char* src = reinterpret_cast<const char*>(p.logits) + (row + e0) * bytes;
+    if (p.type == B2X_F32) {
+#pragma unroll
+      for (int i = 0; i < VPL / 4; ++i) {
+        const float4 f = __ldg(reinterpret_cast<const float4*>(src) + i);
+        l[4 * i] = f.x, l[4 * i + 1] = f.y, l[4 * i + 2] = f.z, l[4 * i + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VPL / 4; ++i) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(src) + i);
+        const uint32_t w[2] = {u.x, u.y};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (p.type == B2X_BF16) {
+            l[4 * i + 2 * j] = bf16lo(w[j]), l[4 * i + 2 * j + 1] = bf16hi(w[j]);
+          } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+            l[4 * i + 2 * j] = f.x, l[4 * i + 2 * j + 1] = f.y;
+          }
+        }
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) l[i] = e0 + i < p.E ? load_f32(p.logits, row + e0 + i, p.type) : -INFINITY;
+}
+
 // The choice in fp64 (rows with values next to a border): lane j < k gets its expert or -1.
 template <int VPL>
-__device__ __noinline__ int choose_exact(const RouteParams& p, const float (&l)[VPL], int lane) {
+__device__ __noinline__ int choose_exact(const RouteParams& p, int64_t row, int lane) {
+  float l[VPL];  // read again: an array handed over would live in memory for every row
+  load_logits<VPL>(p, row, lane, l);
   double c[VPL], s[VPL];
   bool off[VPL];
   double m = -INFINITY, sum = 0.0;
@@ -92,10 +136,10 @@ __device__ __noinline__ int choose_exact(const RouteParams& p, const float (&l)[
     sum += s[i];
   }
   sum = warp_sum(sum);
-  const int gs = p.E / p.groups;
+  const int gs = p.E / p.groups, e0 = lane * VPL;
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
-    const int e = 32 * i + lane;
+    const int e = e0 + i;
     if (!p.sigmoid) s[i] /= sum;
     const float b = p.bias && e < p.E ? p.bias[e] : 0.0f;
     c[i] = p.bias ? s[i] + (double)b : (double)l[i];
@@ -104,49 +148,76 @@ __device__ __noinline__ int choose_exact(const RouteParams& p, const float (&l)[
     if (c[i] != c[i]) c[i] = INFINITY;
     if (s[i] != s[i]) s[i] = INFINITY;
   }
-  if (p.groups > 1) {
-    // every lane keeps the scores of groups lane, lane + 32, ... (groups <= experts <= 1024)
-    bool kept_here[VPL];
+  if (p.groups > 1 && p.lanes_per_group) {
+    // runs of 2^n lanes, as in the kernel: the two largest by exchanges, the rank by counting the better groups
+    double a1 = -INFINITY, a2 = -INFINITY;
+    int n = 0;  // how many there are, up to two
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) kept_here[i] = false;
+    for (int i = 0; i < VPL; ++i)
+      if (!off[i]) {
+        if (n == 0 || s[i] > a1) a2 = a1, a1 = s[i];
+        else if (n == 1 || s[i] > a2) a2 = s[i];
+        n = min(n + 1, 2);
+      }
+    for (int o = 1; o < p.lanes_per_group; o <<= 1) {
+      const double b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
+      const int bn = __shfl_xor_sync(kAll, n, o);
+      const double hi = fmax(a1, b1), lo = fmin(a1, b1);
+      a2 = fmax(lo, fmax(a2, b2));
+      a1 = hi;
+      n = min(n + bn, 2);
+    }
+    const double score = p.top2 && n == 2 ? a1 + a2 : a1;
+    const int g = lane / p.lanes_per_group;
+    int better = 0;
+    for (int i = 0; i < p.groups; ++i) {
+      const double other = __shfl_sync(kAll, score, i * p.lanes_per_group);
+      const int there = __shfl_sync(kAll, n, i * p.lanes_per_group);
+      better += there > 0 && (other > score || (other == score && i < g));
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) off[i] = off[i] || n == 0 || better >= p.top_groups;
+  } else if (p.groups > 1) {
+    // lane keeps the scores of the groups VPL lane .. (groups <= experts <= 32 VPL)
     double gv[VPL];
+    bool kept[VPL];
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) gv[i] = -INFINITY;
+    for (int i = 0; i < VPL; ++i) gv[i] = -INFINITY, kept[i] = false;
     for (int g = 0; g < p.groups; ++g) {
       double total = 0.0;
       bool any = false;
       int skip = -1;
+      const int lo = g * gs - e0, hi = lo + gs;
       for (int round = 0; round < (p.top2 ? 2 : 1); ++round) {
         double v = -INFINITY;
         int at = 0x7fffffff;
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-          const int e = 32 * i + lane;
-          if (!off[i] && e / gs == g && e != skip && (s[i] > v || at == 0x7fffffff)) v = s[i], at = e;
-        }
+        for (int i = 0; i < VPL; ++i)
+          if (!off[i] && i >= lo && i < hi && e0 + i != skip && (s[i] > v || at == 0x7fffffff)) v = s[i], at = e0 + i;
         warp_argmax(v, at);
         if (at != 0x7fffffff) total += v, any = true, skip = at;
       }
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
-        if (32 * i + lane == g && any) gv[i] = total;
+        if (e0 + i == g && any) gv[i] = total;
     }
     for (int n = 0; n < p.top_groups; ++n) {
       double v = -INFINITY;
       int at = 0x7fffffff;
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
-        if (32 * i + lane < p.groups && gv[i] > v) v = gv[i], at = 32 * i + lane;
+        if (e0 + i < p.groups && gv[i] > v) v = gv[i], at = e0 + i;
       warp_argmax(v, at);
       if (at == 0x7fffffff) break;
+      const int lo = at * gs - e0, hi = lo + gs;
 #pragma unroll
       for (int i = 0; i < VPL; ++i) {
-        if (32 * i + lane == at) gv[i] = -INFINITY;
-        if ((32 * i + lane) / gs == at) kept_here[i] = true;
+        if (e0 + i == at) gv[i] = -INFINITY;
+        if (i >= lo && i < hi) kept[i] = true;
       }
     }
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) off[i] = off[i] || !kept_here[i];
+    for (int i = 0; i < VPL; ++i) off[i] = off[i] || !kept[i];
   }
   int mine = -1;
   for (int j = 0; j < p.k; ++j) {
@@ -154,41 +225,48 @@ __device__ __noinline__ int choose_exact(const RouteParams& p, const float (&l)[
     int at = 0x7fffffff;
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
-      if (!off[i] && (c[i] > v || at == 0x7fffffff)) v = c[i], at = 32 * i + lane;
+      if (!off[i] && (c[i] > v || at == 0x7fffffff)) v = c[i], at = e0 + i;
     warp_argmax(v, at);
     if (at == 0x7fffffff) break;
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
-      if (32 * i + lane == at) off[i] = true;
+      if (e0 + i == at) off[i] = true;
     if (lane == j) mine = at;
   }
   return mine;
 }
 
-// Largest key of the warp and the lowest expert that has it.
+// Largest key of the warp and the lowest index that has it (the lanes hold rising runs of indexes).
 template <int VPL>
 __device__ __forceinline__ uint32_t take_max(const uint32_t (&key)[VPL], int lane, int& at) {
   uint32_t best = 0;
 #pragma unroll
   for (int i = 0; i < VPL; ++i) best = max(best, key[i]);
   best = __reduce_max_sync(kAll, best);
-  uint32_t e = 0xffffffffu;
+  int e = 0x7fffffff;
 #pragma unroll
   for (int i = VPL - 1; i >= 0; --i)
-    if (key[i] == best) e = 32 * i + lane;
-  at = (int)__reduce_min_sync(kAll, e);
+    if (key[i] == best) e = lane * VPL + i;
+  at = __shfl_sync(kAll, e, __ffs(__ballot_sync(kAll, e != 0x7fffffff)) - 1);
   return best;
 }
 
+__device__ __forceinline__ void top2_add(float& a, float& b, float v) {  // a >= b; NaN counts as the largest
+  if (!(a >= v) && a == a) b = a, a = v;
+  else if (!(b >= v) && b == b) b = v;
+}
+
 template <int VPL>
-__global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(const RouteParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ? 8 : 4)) moe_route_kernel(const __grid_constant__ RouteParams p) {
+  __shared__ __align__(16) uint32_t pack_key[kRouteWarps][32];
+  __shared__ int pack_at[kRouteWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t t = (int64_t)blockIdx.x * kRouteWarps + warp;
   if (t >= p.tokens) return;
   const int64_t row = t * p.ld;
+  const int e0 = lane * VPL;
   float l[VPL];
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) l[i] = 32 * i + lane < p.E ? load_f32(p.logits, row + 32 * i + lane, p.type) : -INFINITY;
+  load_logits<VPL>(p, row, lane, l);
 
   float m = -INFINITY, sum = 1.0f;
   const bool values = p.bias || (p.groups > 1 && p.top2);  // choices or group scores are sums of rounded numbers
@@ -205,98 +283,182 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(const Route
     if (__any_sync(kAll, nan)) sum = NAN;
   }
   uint32_t key[VPL];
-  float sc[VPL];  // s + b where `values`
+  float sc[VPL];  // what groups are scored by: s + b where `values`, else the logit
   float err = 0.0f;
   if (values) {
     float hi_s = 0.0f, hi_c = 0.0f;
+    const float inv = p.sigmoid ? 0.0f : __fdiv_rn(1.0f, sum);
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      const int e = 32 * i + lane;
-      const float s = l[i] == -INFINITY ? 0.0f : (p.sigmoid ? sigma_fast(l[i]) : __fdividef(__expf(l[i] - m), sum));
-      const float b = p.bias && e < p.E ? __ldg(p.bias + e) : 0.0f;
+      const float s = l[i] == -INFINITY ? 0.0f : (p.sigmoid ? sigma_fast(l[i]) : __expf(l[i] - m) * inv);
+      const float b = p.bias && e0 + i < p.E ? __ldg(p.bias + e0 + i) : 0.0f;
       sc[i] = l[i] == -INFINITY || b == -INFINITY ? -INFINITY : s + b;
       hi_s = fmaxf(hi_s, s);
       if (fabsf(sc[i]) < INFINITY) hi_c = fmaxf(hi_c, fabsf(sc[i]));
-      key[i] = order_key(p.bias ? sc[i] : l[i]);
     }
     err = (0x1p-20f + (p.sigmoid ? 0.0f : (VPL + 5) * 0x1p-24f)) * warp_max(hi_s) + 0x1p-23f * warp_max(hi_c);
   } else {
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) key[i] = order_key(l[i]);
+    for (int i = 0; i < VPL; ++i) sc[i] = l[i];
   }
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) key[i] = order_key(p.bias ? sc[i] : l[i]);
   bool close = false;  // something to be told apart in fp64
   if (p.groups > 1) {
     const int gs = p.E / p.groups;
-    uint32_t gk[VPL];  // lane l: groups l, l + 32, ...
+    if (p.lanes_per_group) {
+      // a group is a run of 2^n lanes: its two largest by n exchanges, its rank by counting the better groups
+      float a = -INFINITY, b = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) gk[i] = 0;
-    for (int g = 0; g < p.groups; ++g) {
-      uint32_t a = 0, b = 0;  // the lane's two largest of the group
-      const int lo = g * gs - lane, hi = lo + gs;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const uint32_t v = 32 * i >= lo && 32 * i < hi ? (p.top2 ? order_key(sc[i]) : key[i]) : 0u;
-        b = max(b, min(a, v));
-        a = max(a, v);
+      for (int i = 0; i < VPL; ++i) top2_add(a, b, sc[i]);
+      for (int o = 1; o < p.lanes_per_group; o <<= 1) {
+        const float a2 = __shfl_xor_sync(kAll, a, o), b2 = __shfl_xor_sync(kAll, b, o);
+        top2_add(a, b, a2);
+        top2_add(a, b, b2);
       }
-      uint32_t score = __reduce_max_sync(kAll, a);
-      if (p.top2) {
-        const uint32_t who = __ballot_sync(kAll, a == score);
-        const uint32_t second = __reduce_max_sync(kAll, lane == __ffs(who) - 1 ? b : a);
-        if (second != 0 && score != 0xffffffffu) score = order_key(key_value(score) + (second == 0xffffffffu ? NAN : key_value(second)));
+      if (p.top2 && b != -INFINITY) a += b;
+      const uint32_t score = order_key(a);
+      const int g = lane / p.lanes_per_group;
+      int better = 0;
+      for (int i = 0; i < p.groups; ++i) {
+        const uint32_t other = __shfl_sync(kAll, score, i * p.lanes_per_group);
+        better += other > score || (other == score && i < g);
+      }
+      const bool kept = score != 0 && g < p.groups && better < p.top_groups;
+      if (values) {  // the border between the groups that stay and those that go
+        const uint32_t last = __reduce_min_sync(kAll, kept ? score : 0xffffffffu);
+        const uint32_t next = __reduce_max_sync(kAll, !kept && g < p.groups ? score : 0u);
+        if (next != 0 && last != 0xffffffffu && next != 0xffffffffu) close = !(key_value(last) - key_value(next) > 6.0f * err);
       }
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
-        if (32 * i + lane == g) gk[i] = score;
-    }
-    bool kept[VPL];
+        if (!kept) key[i] = 0;
+    } else {
+      uint32_t gk[VPL];  // lane l: groups VPL l ..
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) kept[i] = false;
-    uint32_t last = 0;
-    for (int n = 0; n < p.top_groups; ++n) {
-      int at;
-      const uint32_t best = take_max<VPL>(gk, lane, at);
+      for (int i = 0; i < VPL; ++i) gk[i] = 0;
+      for (int g = 0; g < p.groups; ++g) {
+        uint32_t a = 0, b = 0;  // the lane's two largest of the group
+        const int lo = g * gs - e0, hi = lo + gs;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+          const uint32_t v = i >= lo && i < hi ? order_key(sc[i]) : 0u;
+          b = max(b, min(a, v));
+          a = max(a, v);
+        }
+        uint32_t score = __reduce_max_sync(kAll, a);
+        if (p.top2) {
+          const uint32_t who = __ballot_sync(kAll, a == score);
+          const uint32_t second = __reduce_max_sync(kAll, lane == __ffs(who) - 1 ? b : a);
+          if (second != 0 && score != 0xffffffffu) score = order_key(key_value(score) + (second == 0xffffffffu ? NAN : key_value(second)));
+        }
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+          if (e0 + i == g) gk[i] = score;
+      }
+      bool kept[VPL];
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) kept[i] = false;
+      uint32_t last = 0;
+      for (int n = 0; n < p.top_groups; ++n) {
+        int at;
+        const uint32_t best = take_max<VPL>(gk, lane, at);
+        if (best == 0) break;
+        last = best;
+        const int lo = at * gs - e0, hi = lo + gs;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+          if (e0 + i == at) gk[i] = 0;
+          if (i >= lo && i < hi) kept[i] = true;
+        }
+      }
+      if (values && last != 0) {
+        int at;
+        const uint32_t next = take_max<VPL>(gk, lane, at);
+        if (next != 0 && last != 0xffffffffu && next != 0xffffffffu) close = !(key_value(last) - key_value(next) > 6.0f * err);
+      }
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (!kept[i]) key[i] = 0;
+    }
+  }
+
+  // The choices in falling order, one to a lane: lane j has the (j + 1)-th key and its expert; key 0: none.
+  uint32_t my_key = 0;
+  int at = -1;
+  uint32_t bound = 1;
+  if (VPL > 1 && p.k < 32) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) top = max(top, key[i]);
+    for (int j = 0; j <= p.k; ++j) {
+      bound = __reduce_max_sync(kAll, top);
+      if (top == bound) top = 0;
+    }
+    bound = max(bound, 1u);
+  }
+  uint32_t in = 0;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) in |= key[i] >= bound ? 1u << i : 0u;
+  int slot = __popc(in), n = slot;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(kAll, n, o);
+    if (lane >= o) n += v;
+  }
+  slot = n - slot;
+  n = __shfl_sync(kAll, n, 31);
+  if (n <= 32) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (in >> i & 1) {
+        pack_key[warp][slot] = key[i];
+        pack_at[warp][slot++] = e0 + i;
+      }
+    __syncwarp();
+    if (lane < n) my_key = pack_key[warp][lane], at = pack_at[warp][lane];
+    int better = 0;  // larger keys, and equal ones of lower index
+    for (int j = 0; j < n; j += 4) {
+      const uint4 k4 = *reinterpret_cast<const uint4*>(&pack_key[warp][j]);
+      const uint32_t other[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (j + u < n) better += other[u] > (j + u < lane ? my_key - 1 : my_key);
+    }
+    __syncwarp();
+    if (lane < n) pack_key[warp][better] = my_key, pack_at[warp][better] = at;
+    __syncwarp();
+    my_key = lane < n ? pack_key[warp][lane] : 0;
+    at = lane < n ? pack_at[warp][lane] : -1;
+  } else {  // more candidates than lanes: one after the other
+    for (int j = 0; j <= min(p.k, 31); ++j) {
+      int e;
+      const uint32_t best = take_max<VPL>(key, lane, e);
       if (best == 0) break;
-      last = best;
-      const int lo = at * gs - lane, hi = lo + gs;
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        if (32 * i + lane == at) gk[i] = 0;
-        if (32 * i >= lo && 32 * i < hi) kept[i] = true;
-      }
+      for (int i = 0; i < VPL; ++i)
+        if (e0 + i == e) key[i] = 0;
+      if (lane == j) my_key = best, at = e;
     }
-    if (values && last != 0) {  // the border between the groups that stay and those that go
-      int at;
-      const uint32_t next = take_max<VPL>(gk, lane, at);
-      if (next != 0 && last != 0xffffffffu && next != 0xffffffffu) close = !(key_value(last) - key_value(next) > 6.0f * err);
+    if (p.k == 32 && p.bias) {  // no lane is left to hold the 33rd: compare it here
+      int e;
+      const uint32_t best = take_max<VPL>(key, lane, e);
+      const uint32_t last = __shfl_sync(kAll, my_key, 31);
+      if (best != 0 && last != 0xffffffffu && !(key_value(last) - key_value(best) > 2.0f * err)) close = true;
     }
-#pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (!kept[i]) key[i] = 0;
   }
-  int mine = -1;
-  uint32_t before = 0;
-  int before_at = 0;
-  for (int j = 0; j < p.k + (p.bias ? 1 : 0); ++j) {
-    int at;
-    const uint32_t best = take_max<VPL>(key, lane, at);
-    if (best == 0) break;
-    if (p.bias && j > 0 && before != 0xffffffffu) {
-      // equal logits with equal biases are a true tie, which the index decides
-      const bool near = !(key_value(before) - key_value(best) > 2.0f * err);
-      if (near) {
-        const float la = load_f32(p.logits, row + before_at, p.type), lb = load_f32(p.logits, row + at, p.type);
-        if (!(la == lb && __ldg(p.bias + before_at) == __ldg(p.bias + at))) close = true;
-      }
+  int mine = lane < p.k ? at : -1;
+  if (p.bias) {
+    // neighbours in the order that fp32 cannot tell apart, unless logits and biases are the same: then the index decides
+    const uint32_t next_key = __shfl_down_sync(kAll, my_key, 1);
+    const int next_at = __shfl_down_sync(kAll, at, 1);
+    if (lane < p.k && lane < 31 && my_key != 0 && next_key != 0 && my_key != 0xffffffffu && next_key != 0xffffffffu &&
+        !(key_value(my_key) - key_value(next_key) > 2.0f * err)) {
+      const float la = load_f32(p.logits, row + at, p.type), lb = load_f32(p.logits, row + next_at, p.type);
+      if (!(la == lb && __ldg(p.bias + at) == __ldg(p.bias + next_at))) close = true;
     }
-    before = best;
-    before_at = at;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (32 * i + lane == at) key[i] = 0;
-    if (lane == j && j < p.k) mine = at;
   }
-  if (close) mine = choose_exact<VPL>(p, l, lane);  // uniform over the warp
+  if (__any_sync(kAll, close)) mine = choose_exact<VPL>(p, row, lane);
 
   // lane j: the weight of its expert
   float w = 0.0f;
@@ -330,6 +492,30 @@ __device__ __forceinline__ void store_f32(void* p, int64_t i, int type, float v)
     reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
+// VPL consecutive gradients of a row.
+template <int VPL>
+__device__ __forceinline__ void store_logits(const RouteParams& p, int64_t row, int lane, const float (&v)[VPL]) {
+  const int e0 = lane * VPL;
+  if (VPL % 4 == 0 && p.vec_d && e0 + VPL <= p.E) {
+    char* dst = reinterpret_cast<char*>(p.d_logits) + (row + e0) * (p.type == B2X_F32 ? 4 : 2);
+#pragma unroll
+    for (int i = 0; i < VPL / 4; ++i) {
+      if (p.type == B2X_F32) {
+        reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      } else if (p.type == B2X_BF16) {
+        reinterpret_cast<uint2*>(dst)[i] = make_uint2(pack_bf16x2(v[4 * i], v[4 * i + 1]), pack_bf16x2(v[4 * i + 2], v[4 * i + 3]));
+      } else {
+        const __half2 a = __floats2half2_rn(v[4 * i], v[4 * i + 1]), b = __floats2half2_rn(v[4 * i + 2], v[4 * i + 3]);
+        reinterpret_cast<uint2*>(dst)[i] = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < VPL; ++i)
+    if (e0 + i < p.E) store_f32(p.d_logits, row + e0 + i, p.type, v[i]);
+}
+
 // d_logits of one token per warp.  With w_j = scale s_j (/ S, S = sum of the chosen s):
 //   ds_j = scale d_j                              or  scale (d_j - sum_i d_i s_i / S) / S
 //   sigmoid:  dl_e = ds_e s_e (1 - s_e)
@@ -338,7 +524,7 @@ __device__ __forceinline__ void store_f32(void* p, int64_t i, int type, float v)
 // An expert named in two slots gets the sum of both.  The rest of the row is the dense part (0 except for the
 // softmax over all experts), stored first; the chosen ones are stored over it after a __syncwarp.
 template <int VPL>
-__global__ void __launch_bounds__(kRouteWarps * 32) moe_route_backward_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(kRouteWarps * 32) moe_route_backward_kernel(const __grid_constant__ RouteParams p) {
   const int lane = threadIdx.x & 31;
   const int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
   if (t >= p.tokens) return;
@@ -356,11 +542,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_backward_kernel(co
   if (dense) {
     float l[VPL];
     float m = -INFINITY, sum = 0.0f;
+    load_logits<VPL>(p, row, lane, l);
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      l[i] = 32 * i + lane < p.E ? load_f32(p.logits, row + 32 * i + lane, p.type) : -INFINITY;
-      m = fmaxf(m, l[i]);
-    }
+    for (int i = 0; i < VPL; ++i) m = fmaxf(m, l[i]);
     m = warp_max(m);
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
@@ -372,8 +556,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_backward_kernel(co
     const float s = at >= 0 ? __expf(lm - m) * r : 0.0f;
     const float mean = warp_sum(at >= 0 ? s * d : 0.0f);
 #pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (32 * i + lane < p.E) store_f32(p.d_logits, t * p.ld_d + 32 * i + lane, p.type, -l[i] * r * mean);
+    for (int i = 0; i < VPL; ++i) l[i] = -l[i] * r * mean;
+    store_logits<VPL>(p, t * p.ld_d, lane, l);
     float all = 0.0f;  // of every slot that names this lane's expert
     for (int j = 0; j < p.k; ++j) {
       const int aj = __shfl_sync(kAll, at, j);
@@ -382,9 +566,10 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_backward_kernel(co
     }
     mine = s * (all - mean);
   } else {
+    float zero[VPL];
 #pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (32 * i + lane < p.E) store_f32(p.d_logits, t * p.ld_d + 32 * i + lane, p.type, 0.0f);
+    for (int i = 0; i < VPL; ++i) zero[i] = 0.0f;
+    store_logits<VPL>(p, t * p.ld_d, lane, zero);
     float dl = 0.0f;  // this slot's part
     if (p.sigmoid) {
       const float s = at >= 0 ? sigma_fast(lm) : 0.0f;
@@ -415,20 +600,38 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_backward_kernel(co
 }
 
 template <int BACKWARD>
-static cudaError_t launch_route(const RouteParams& p, cudaStream_t st) {
+static cudaError_t launch_route(RouteParams p, cudaStream_t st) {
   const unsigned grid = (unsigned)((p.tokens + kRouteWarps - 1) / kRouteWarps);
   const int per = (p.E + 31) / 32;
+  static constexpr int kWidths[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 32};
+  int vpl = 1;
+  for (int w : kWidths) {
+    vpl = w;
+    if (w >= per) break;
+  }
+  const int bytes = 4 * (p.type == B2X_F32 ? 4 : 2);  // of four values
+  p.vec = (uintptr_t)p.logits % bytes == 0 && p.ld % 4 == 0;
+  p.vec_d = (uintptr_t)p.d_logits % bytes == 0 && p.ld_d % 4 == 0;
+  const int gs = p.E / p.groups, lanes = gs / vpl;
+  p.lanes_per_group = gs % vpl == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
 #define B2X_ROUTE(V)                                                       \
   if constexpr (BACKWARD)                                                  \
     moe_route_backward_kernel<V><<<grid, kRouteWarps * 32, 0, st>>>(p);    \
   else                                                                     \
     moe_route_kernel<V><<<grid, kRouteWarps * 32, 0, st>>>(p)
-  if (per <= 1) { B2X_ROUTE(1); }
-  else if (per <= 2) { B2X_ROUTE(2); }
-  else if (per <= 4) { B2X_ROUTE(4); }
-  else if (per <= 8) { B2X_ROUTE(8); }
-  else if (per <= 16) { B2X_ROUTE(16); }
-  else { B2X_ROUTE(32); }
+  switch (vpl) {
+    case 1: B2X_ROUTE(1); break;
+    case 2: B2X_ROUTE(2); break;
+    case 3: B2X_ROUTE(3); break;
+    case 4: B2X_ROUTE(4); break;
+    case 5: B2X_ROUTE(5); break;
+    case 6: B2X_ROUTE(6); break;
+    case 8: B2X_ROUTE(8); break;
+    case 10: B2X_ROUTE(10); break;
+    case 12: B2X_ROUTE(12); break;
+    case 16: B2X_ROUTE(16); break;
+    default: B2X_ROUTE(32); break;
+  }
 #undef B2X_ROUTE
   note_launch(1);
   return cudaGetLastError();
