@@ -14,7 +14,7 @@
 namespace b2x {
 
 constexpr int kEbThreads = 256;
-constexpr int kEbUnroll = 4;  // rows in flight per thread
+constexpr int kEbUnroll = 2;  // rows in flight per thread (1 to 4 with 2 to 6 CTAs per SM: 126 us here, 145 to 275 elsewhere)
 
 struct EpiBwdParams {
   const void* grad;
@@ -42,7 +42,7 @@ __device__ __forceinline__ Piece<T, V> load_plain(const T* p) {
 
 // Grid: x = column blocks * cluster size; the CTAs of a cluster share their columns and split the rows.
 template <typename T, int V, int ACT, int TX>
-__global__ void __launch_bounds__(kEbThreads) epilogue_backward_kernel(const EpiBwdParams p, int splits) {
+__global__ void __launch_bounds__(kEbThreads, 4) epilogue_backward_kernel(const EpiBwdParams p, int splits) {
   constexpr int TY = kEbThreads / TX;
   __shared__ float part[TY][TX * V + 1];
   const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
@@ -72,11 +72,28 @@ __global__ void __launch_bounds__(kEbThreads) epilogue_backward_kernel(const Epi
         const int64_t ru = r + (int64_t)u * TY;
         if (ru < r1) {
           Piece<T, V> ov;
+          if constexpr (V == 1) {
+            float d, none;
+            unpair(act_slope<ACT>(pair(to_f32(zv[u].e[0]))), d, none);
+            d *= to_f32(gv[u].e[0]);
+            sum[0] += d;
+            ov.e[0] = from_f32<T>(d);
+          } else {
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float d = to_f32(gv[u].e[i]) * act_slope<ACT>(to_f32(zv[u].e[i]));
-            sum[i] += d;
-            ov.e[i] = from_f32<T>(d);
+            for (int i = 0; i < V; i += 2) {
+              const Pair z2 = pair(to_f32(zv[u].e[i]), to_f32(zv[u].e[i + 1]));
+              const Pair d2 = mul2(pair(to_f32(gv[u].e[i]), to_f32(gv[u].e[i + 1])), act_slope<ACT>(z2));
+              float a, b;
+              unpair(add2(pair(sum[i], sum[i + 1]), d2), sum[i], sum[i + 1]);
+              unpair(d2, a, b);
+              if constexpr (__is_same(T, __nv_bfloat16)) {
+                const uint32_t w = pack_bf16x2(a, b);
+                memcpy(&ov.e[i], &w, 4);
+              } else {
+                ov.e[i] = from_f32<T>(a);
+                ov.e[i + 1] = from_f32<T>(b);
+              }
+            }
           }
           store_piece<T, V>(o + ru * p.ld_out, ov);
         }
@@ -141,9 +158,13 @@ static cudaError_t launch_epi_bwd_t(const EpiBwdParams& p, int num_sms, cudaStre
 template <typename T, int ACT>
 static cudaError_t launch_epi_bwd_act(const EpiBwdParams& p, bool vec, int num_sms, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  // Narrow matrices take fewer threads side by side, so that none idles past the last column.
+  // Threads side by side: 32 for whole 512-byte runs, fewer where the column blocks, each split over at most 8 CTAs, would
+  // not give every SM two (8192 x 1024 on 32: 82 us).
   if (!vec) return launch_epi_bwd_t<T, 1, ACT, 32>(p, num_sms, st);
-  return p.cols <= 8 * V ? launch_epi_bwd_t<T, V, ACT, 8>(p, num_sms, st) : launch_epi_bwd_t<T, V, ACT, 32>(p, num_sms, st);
+  const int64_t runs = (p.cols + V - 1) / V;
+  if (runs / 32 * 8 >= 2 * num_sms) return launch_epi_bwd_t<T, V, ACT, 32>(p, num_sms, st);
+  if (runs / 8 * 8 >= 2 * num_sms) return launch_epi_bwd_t<T, V, ACT, 8>(p, num_sms, st);
+  return launch_epi_bwd_t<T, V, ACT, 4>(p, num_sms, st);
 }
 
 template <typename T>

@@ -232,7 +232,7 @@ __device__ __forceinline__ void tok_tile(const TokParams& p, const TokCols& c, u
 
 __device__ __forceinline__ float tok_swiglu(float g, float u, float alpha) {
   g = __fmul_rn(g, alpha);
-  return __fmul_rn(__fdividef(g, 1.0f + __expf(-g)), __fmul_rn(u, alpha));
+  return __fmul_rn(__fmul_rn(g, sigma_fast(g)), __fmul_rn(u, alpha));
 }
 
 // The same for a SwiGLU tile, whose 128 weight rows alternate 16 gate and 16 up rows: 64 columns of h.  Half a warp per

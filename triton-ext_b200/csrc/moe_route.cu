@@ -11,7 +11,7 @@
 //
 // What is compared.  Without a bias s is monotone in the logit, so the logits themselves are the keys and the choice is
 // exact.  With a bias (and for sums of two) the keys are fp32 values of s + b, each off by at most
-// `err` = (2^-20 + softmax: (VPL + 5) 2^-24) max s + 2^-23 max |s + b|: the fast exponential and division together stay
+// `err` = (2^-20 + softmax: (VPL + 5) 2^-24) max s + 2^-23 max |s + b|: the approximate exponential and reciprocal together stay
 // below 2^-20 relative, the softmax's sum adds VPL + 5 roundings, and s + b is rounded once.  A row whose chosen values
 // lie closer than 2 err, or whose group scores (sums of two, 3 err each) lie closer than 6 err at the border, is chosen
 // again in fp64 (choose_exact): the choice is right to fp64, at the speed of fp32 for nearly all rows.
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
     m = warp_max(m);
     sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) sum += l[i] == -INFINITY ? 0.0f : __expf(l[i] - m);
+    for (int i = 0; i < VPL; ++i) sum += l[i] == -INFINITY ? 0.0f : exp_approx(l[i] - m);
     sum = warp_sum(sum);
     if (__any_sync(kAll, nan)) sum = NAN;
   }
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
     const float inv = p.sigmoid ? 0.0f : __fdiv_rn(1.0f, sum);
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      const float s = l[i] == -INFINITY ? 0.0f : (p.sigmoid ? sigma_fast(l[i]) : __expf(l[i] - m) * inv);
+      const float s = l[i] == -INFINITY ? 0.0f : (p.sigmoid ? sigma_fast(l[i]) : exp_approx(l[i] - m) * inv);
       const float b = p.bias && e0 + i < p.E ? __ldg(p.bias + e0 + i) : 0.0f;
       sc[i] = l[i] == -INFINITY || b == -INFINITY ? -INFINITY : s + b;
       hi_s = fmaxf(hi_s, s);
@@ -471,11 +471,11 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
     }
   } else if (p.renorm) {  // softmax over the chosen ones: the common factor cancels
     const float top = warp_max(lm);
-    if (mine >= 0) w = __expf(lm - top);
+    if (mine >= 0) w = exp_approx(lm - top);
     const float total = warp_sum(w);
     w = mine >= 0 ? __fdiv_rn(w, total) : 0.0f;
   } else if (mine >= 0) {
-    w = __fdiv_rn(__expf(lm - m), sum);
+    w = __fdiv_rn(exp_approx(lm - m), sum);
   }
   if (lane < p.k) {
     p.weights[t * p.k + lane] = mine >= 0 ? w * p.scale : 0.0f;
@@ -548,12 +548,12 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_backward_kernel(co
     m = warp_max(m);
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      l[i] = l[i] == -INFINITY ? 0.0f : __expf(l[i] - m);
+      l[i] = l[i] == -INFINITY ? 0.0f : exp_approx(l[i] - m);
       sum += l[i];
     }
     sum = warp_sum(sum);
     const float r = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
-    const float s = at >= 0 ? __expf(lm - m) * r : 0.0f;
+    const float s = at >= 0 ? exp_approx(lm - m) * r : 0.0f;
     const float mean = warp_sum(at >= 0 ? s * d : 0.0f);
 #pragma unroll
     for (int i = 0; i < VPL; ++i) l[i] = -l[i] * r * mean;
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_backward_kernel(co
       }
     } else {
       const float top = warp_max(lm);
-      float pr = at >= 0 ? __expf(lm - top) : 0.0f;
+      float pr = at >= 0 ? exp_approx(lm - top) : 0.0f;
       const float total = warp_sum(pr);
       pr = at >= 0 ? __fdiv_rn(pr, total) : 0.0f;
       const float mean = warp_sum(at >= 0 ? pr * d : 0.0f);

@@ -23,6 +23,10 @@ namespace b2x {
 
 constexpr int kRowThreads = 128;
 constexpr int kFusedPairs = 2048;   // pairs that a CTA counts by itself
+#ifndef CCTAS
+#define CCTAS 4736
+#endif
+constexpr int kCombineCtas = CCTAS;
 constexpr int kPlanCtas = 8;
 constexpr int kPlanThreads = 512;
 constexpr int kPlanWarps = kPlanThreads / 32;
@@ -136,30 +140,34 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
   cluster_sync();  // peers may still read this CTA's totals
 }
 
-// 16 consecutive values of x as fp32 pairs.
-__device__ __forceinline__ void load16(const DispatchParams& p, int64_t at, int64_t col, float (&v)[16]) {
+// 16 consecutive values of a row as they are stored: 16 or 8 registers.
+template <typename T>
+struct Raw16 {
+  uint4 v[sizeof(T)];
+};
+template <typename T>
+__device__ __forceinline__ Raw16<T> load16(const DispatchParams& p, int64_t at, int64_t col) {
+  Raw16<T> r;
+  const T* s = reinterpret_cast<const T*>(p.x) + at + col;
   if (p.vec && col + 16 <= p.cols) {
-    if (p.x_f32) {
-      const float4* s = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + at + col);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 f = __ldcs(s + i);
-        v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
-      }
-    } else {
-      const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + at + col);
+    for (int i = 0; i < (int)sizeof(T); ++i) r.v[i] = __ldcs(reinterpret_cast<const uint4*>(s) + i);
+  } else {
+    T e[16];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint4 u = __ldcs(s + i);
-        v[8 * i] = bf16lo(u.x), v[8 * i + 1] = bf16hi(u.x), v[8 * i + 2] = bf16lo(u.y), v[8 * i + 3] = bf16hi(u.y);
-        v[8 * i + 4] = bf16lo(u.z), v[8 * i + 5] = bf16hi(u.z), v[8 * i + 6] = bf16lo(u.w), v[8 * i + 7] = bf16hi(u.w);
-      }
-    }
-    return;
+    for (int i = 0; i < 16; ++i) e[i] = col + i < p.cols ? s[i] : T(0);
+    memcpy(&r, e, sizeof(r));
   }
+  return r;
+}
+__device__ __forceinline__ void unpack16(const Raw16<float>& r, float (&v)[16]) { memcpy(v, &r, 64); }
+__device__ __forceinline__ void unpack16(const Raw16<uint16_t>& r, float (&v)[16]) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    v[i] = col + i < p.cols ? load_f32(p.x, at + col + i, p.x_f32 ? B2X_F32 : B2X_BF16) : 0.0f;
+  for (int i = 0; i < 2; ++i) {
+    const uint4 u = r.v[i];
+    v[8 * i] = bf16lo(u.x), v[8 * i + 1] = bf16hi(u.x), v[8 * i + 2] = bf16lo(u.y), v[8 * i + 3] = bf16hi(u.y);
+    v[8 * i + 4] = bf16lo(u.z), v[8 * i + 5] = bf16hi(u.z), v[8 * i + 6] = bf16lo(u.w), v[8 * i + 7] = bf16hi(u.w);
+  }
 }
 
 template <int FP8>
@@ -184,7 +192,7 @@ __device__ __forceinline__ void store16(const DispatchParams& p, const float (&v
 
 // One CTA per token.  NV: 16-value pieces that a thread holds in registers (cols <= kRowThreads * 16 * NV); NV = 0:
 // longer rows, read a second time (from L2) for the cast.
-template <int NV, int FP8>
+template <typename T, int NV, int FP8>
 __global__ void __launch_bounds__(kRowThreads) moe_dispatch_kernel(const DispatchParams p) {
   extern __shared__ int row_smem[];  // fused: cnt[E + 1]; always: row[k]
   __shared__ int warp_part[kRowThreads / 32];
@@ -193,12 +201,13 @@ __global__ void __launch_bounds__(kRowThreads) moe_dispatch_kernel(const Dispatc
   int* row = row_smem;
   int* cnt = row_smem + p.k;
   const int64_t at = t * p.ld_x;
-  float v[NV ? NV : 1][16];
+  Raw16<T> raw[NV ? NV : 1];
+  float v[16];
   float amax = 0.0f;
   // the row's loads are issued before the ranking
   if (NV) {
 #pragma unroll
-    for (int n = 0; n < NV; ++n) load16(p, at, (int64_t)(n * kRowThreads + threadIdx.x) * 16, v[n]);
+    for (int n = 0; n < NV; ++n) raw[n] = load16<T>(p, at, (int64_t)(n * kRowThreads + threadIdx.x) * 16);
   }
   if (p.fused) {
     const int pairs = (int)(p.tokens * p.k), own = (int)(t * p.k);
@@ -228,14 +237,16 @@ __global__ void __launch_bounds__(kRowThreads) moe_dispatch_kernel(const Dispatc
   if (!p.given) {
     if (NV) {
 #pragma unroll
-      for (int n = 0; n < NV; ++n)
+      for (int n = 0; n < NV; ++n) {
+        unpack16(raw[n], v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) amax = absmax_xs(amax, v[n][i]);
+        for (int i = 0; i < 16; ++i) amax = absmax_xs(amax, v[i]);
+      }
     } else {
       for (int64_t c = (int64_t)threadIdx.x * 16; c < p.cols; c += kRowThreads * 16) {
-        load16(p, at, c, v[0]);
+        unpack16(load16<T>(p, at, c), v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) amax = absmax_xs(amax, v[0][i]);
+        for (int i = 0; i < 16; ++i) amax = absmax_xs(amax, v[i]);
       }
     }
     amax = fabsf(amax);
@@ -258,24 +269,25 @@ __global__ void __launch_bounds__(kRowThreads) moe_dispatch_kernel(const Dispatc
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int64_t c = (int64_t)(n * kRowThreads + threadIdx.x) * 16;
-      if (c < p.cols) store16<FP8>(p, v[n], inv, c, row, p.k);
+      unpack16(raw[n], v);
+      if (c < p.cols) store16<FP8>(p, v, inv, c, row, p.k);
     }
   } else {
     for (int64_t c = (int64_t)threadIdx.x * 16; c < p.cols; c += kRowThreads * 16) {
-      load16(p, at, c, v[0]);
-      store16<FP8>(p, v[0], inv, c, row, p.k);
+      unpack16(load16<T>(p, at, c), v);
+      store16<FP8>(p, v, inv, c, row, p.k);
     }
   }
 }
 
-template <int FP8>
+template <typename T, int FP8>
 static void launch_dispatch_rows(const DispatchParams& p, size_t smem, cudaStream_t st) {
   const int64_t per = (p.cols + kRowThreads * 16 - 1) / (kRowThreads * 16);
   const unsigned grid = (unsigned)p.tokens;
-  if (per <= 1) moe_dispatch_kernel<1, FP8><<<grid, kRowThreads, smem, st>>>(p);
-  else if (per <= 2) moe_dispatch_kernel<2, FP8><<<grid, kRowThreads, smem, st>>>(p);
-  else if (per <= 4) moe_dispatch_kernel<4, FP8><<<grid, kRowThreads, smem, st>>>(p);
-  else moe_dispatch_kernel<0, FP8><<<grid, kRowThreads, smem, st>>>(p);
+  if (per <= 1) moe_dispatch_kernel<T, 1, FP8><<<grid, kRowThreads, smem, st>>>(p);
+  else if (per <= 2) moe_dispatch_kernel<T, 2, FP8><<<grid, kRowThreads, smem, st>>>(p);
+  else if (per <= 4) moe_dispatch_kernel<T, 4, FP8><<<grid, kRowThreads, smem, st>>>(p);
+  else moe_dispatch_kernel<T, 0, FP8><<<grid, kRowThreads, smem, st>>>(p);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- combine
@@ -330,6 +342,24 @@ __device__ __forceinline__ Piece<T, V> load_piece(const T* p) {
     return r;
   }
 }
+// The piece, or zeros where `in` is false: a predicate, not a branch, so that several loads go out together.
+template <typename T, int V>
+__device__ __forceinline__ Piece<T, V> load_piece_if(bool in, const T* p) {
+  Piece<T, V> r;
+  if constexpr (V == 1) {
+    r.e[0] = in ? *p : from_f32<T>(0.0f);
+  } else {
+    uint4 u;
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+        "@q ld.global.cs.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+        : "=&r"(u.x), "=&r"(u.y), "=&r"(u.z), "=&r"(u.w)
+        : "l"(p), "r"((int)in));
+    memcpy(&r, &u, 16);
+  }
+  return r;
+}
 template <typename T, int V>
 __device__ __forceinline__ void store_piece(T* p, const Piece<T, V>& v) {
   if constexpr (V == 1) {
@@ -341,45 +371,45 @@ __device__ __forceinline__ void store_piece(T* p, const Piece<T, V>& v) {
   }
 }
 
-// One CTA per (token, kRowThreads * V columns).
-template <typename T, int V>
-__global__ void __launch_bounds__(kRowThreads) moe_combine_kernel(const CombineParams p) {
-  const uint32_t per = (uint32_t)((p.cols + kRowThreads * V - 1) / (kRowThreads * V));  // CTAs of a token: < 2^31 in all
-  const int64_t t = blockIdx.x / per;
-  const int64_t c = ((int64_t)(blockIdx.x % per) * kRowThreads + threadIdx.x) * V;
-  if (c >= p.cols) return;
-  const T* y = reinterpret_cast<const T*>(p.y);
-  float acc[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+// A CTA takes a token's columns in steps of kRowThreads * V, `per` CTAs side by side.  MANY: more than 8 slots, their rows
+// and weights read again for every step.
+template <typename T, int V, bool MANY>
+__global__ void __launch_bounds__(kRowThreads) moe_combine_kernel(const CombineParams p, uint32_t per) {
   constexpr int U = 8;  // rows in flight
-  for (int j0 = 0; j0 < p.k; j0 += U) {
-    Piece<T, V> v[U];
-    float w[U];
+  const int64_t t = blockIdx.x / per;
+  const T* y = reinterpret_cast<const T*>(p.y);
+  const int64_t step = (int64_t)per * kRowThreads * V;
+  int r[U];
+  float w[U];
+  auto slots = [&](int j0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t r = j0 + u < p.k ? __ldg(p.rows + t * p.k + j0 + u) : -1;
-      const bool in = r >= 0 && r < p.y_rows;
-      w[u] = in ? (p.weights ? __ldg(p.weights + t * p.k + j0 + u) : 1.0f) : 0.0f;
-      if (in)
-        v[u] = load_piece<T, V>(y + r * p.ld_y + c);
-      else
-        v[u] = Piece<T, V>{};
+      r[u] = j0 + u < p.k ? __ldg(p.rows + t * p.k + j0 + u) : -1;
+      if (r[u] >= p.y_rows) r[u] = -1;
+      w[u] = r[u] < 0 ? 0.0f : (p.weights ? __ldg(p.weights + t * p.k + j0 + u) : 1.0f);
     }
+  };
+  if (!MANY) slots(0);
+  for (int64_t c = ((int64_t)(blockIdx.x % per) * kRowThreads + threadIdx.x) * V; c < p.cols; c += step) {
+    float acc[V];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+    const Piece<T, V> res = load_piece_if<T, V>(p.residual != nullptr, reinterpret_cast<const T*>(p.residual) + t * p.ld_res + c);
+    for (int j0 = 0; j0 < (MANY ? p.k : 1); j0 += U) {
+      if (MANY) slots(j0);
+      Piece<T, V> v[U];
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] = fmaf(w[u], to_f32(v[u].e[i]), acc[i]);
+      for (int u = 0; u < U; ++u) v[u] = load_piece_if<T, V>(r[u] >= 0, y + (int64_t)r[u] * p.ld_y + c);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = fmaf(w[u], to_f32(v[u].e[i]), acc[i]);
+    }
+    Piece<T, V> o;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o.e[i] = from_f32<T>(acc[i] + to_f32(res.e[i]));
+    store_piece<T, V>(reinterpret_cast<T*>(p.out) + t * p.ld_out + c, o);
   }
-  if (p.residual) {
-    const Piece<T, V> r = load_piece<T, V>(reinterpret_cast<const T*>(p.residual) + t * p.ld_res + c);
-#pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] += to_f32(r.e[i]);
-  }
-  Piece<T, V> o;
-#pragma unroll
-  for (int i = 0; i < V; ++i) o.e[i] = from_f32<T>(acc[i]);
-  store_piece<T, V>(reinterpret_cast<T*>(p.out) + t * p.ld_out + c, o);
 }
 
 // One CTA per token; KC slots at a time (their dot products stay in registers).
@@ -392,7 +422,7 @@ __global__ void __launch_bounds__(kRowThreads) moe_combine_backward_kernel(const
   const T* g = reinterpret_cast<const T*>(p.grad) + t * p.ld_grad;
   T* dy = reinterpret_cast<T*>(p.out);
   for (int j0 = 0; j0 < p.k; j0 += KC) {
-    int64_t r[KC];
+    int r[KC];
     float w[KC], dot[KC];
 #pragma unroll
     for (int u = 0; u < KC; ++u) {
@@ -405,10 +435,7 @@ __global__ void __launch_bounds__(kRowThreads) moe_combine_backward_kernel(const
       Piece<T, V> v[KC];
 #pragma unroll
       for (int u = 0; u < KC; ++u)
-        if (r[u] >= 0)
-          v[u] = load_piece<T, V>(y + r[u] * p.ld_y + c);
-        else
-          v[u] = Piece<T, V>{};
+        v[u] = load_piece_if<T, V>(r[u] >= 0, y + (int64_t)r[u] * p.ld_y + c);
       const Piece<T, V> gv = load_piece<T, V>(g + c);
       float gf[V];
 #pragma unroll
@@ -422,7 +449,7 @@ __global__ void __launch_bounds__(kRowThreads) moe_combine_backward_kernel(const
           dot[u] = fmaf(gf[i], to_f32(v[u].e[i]), dot[u]);
           o.e[i] = from_f32<T>(w[u] * gf[i]);
         }
-        store_piece<T, V>(dy + r[u] * p.ld_out + c, o);
+        store_piece<T, V>(dy + (int64_t)r[u] * p.ld_out + c, o);
       }
     }
 #pragma unroll
@@ -453,12 +480,17 @@ static cudaError_t launch_combine_t(const CombineParams& p, bool vec, cudaStream
       moe_combine_backward_kernel<T, 1, 8><<<grid, kRowThreads, 0, st>>>(p);
   } else {
     const int v = vec ? V : 1;
-    const int64_t per = (p.cols + kRowThreads * v - 1) / (kRowThreads * v);
+    // CTAs side by side on a token: all its steps while the tokens are few, fewer once they fill the GPU
+    uint32_t per = (uint32_t)((p.cols + kRowThreads * v - 1) / (kRowThreads * v));
+    while (per > 1 && p.tokens * per > kCombineCtas) per = (per + 1) / 2;
     const unsigned grid = (unsigned)(p.tokens * per);
-    if (vec)
-      moe_combine_kernel<T, V><<<grid, kRowThreads, 0, st>>>(p);
-    else
-      moe_combine_kernel<T, 1><<<grid, kRowThreads, 0, st>>>(p);
+    if (vec) {
+      p.k > 8 ? moe_combine_kernel<T, V, true><<<grid, kRowThreads, 0, st>>>(p, per)
+              : moe_combine_kernel<T, V, false><<<grid, kRowThreads, 0, st>>>(p, per);
+    } else {
+      p.k > 8 ? moe_combine_kernel<T, 1, true><<<grid, kRowThreads, 0, st>>>(p, per)
+              : moe_combine_kernel<T, 1, false><<<grid, kRowThreads, 0, st>>>(p, per);
+    }
   }
   note_launch(1);
   return cudaGetLastError();
@@ -529,10 +561,10 @@ extern "C" B2X_API b2x_status b2x_moe_dispatch(const b2x_moe_dispatch_args* a, v
     if (e != cudaSuccess) return cuda_fail(e, "b2x_moe_dispatch launch (plan)");
   }
   const size_t smem = (size_t)(p.k + (p.fused ? p.E + 1 : 0)) * 4;
-  if (a->q_type == B2X_E5M2)
-    launch_dispatch_rows<1>(p, smem, st);
+  if (p.x_f32)
+    a->q_type == B2X_E5M2 ? launch_dispatch_rows<float, 1>(p, smem, st) : launch_dispatch_rows<float, 0>(p, smem, st);
   else
-    launch_dispatch_rows<0>(p, smem, st);
+    a->q_type == B2X_E5M2 ? launch_dispatch_rows<uint16_t, 1>(p, smem, st) : launch_dispatch_rows<uint16_t, 0>(p, smem, st);
   note_launch(1);
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? B2X_OK : cuda_fail(e, "b2x_moe_dispatch launch");
