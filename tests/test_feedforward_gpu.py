@@ -792,10 +792,11 @@ def test_layer(T, E, H, I, k):
     check(out, ref, tol + rounded(BF, ref.abs() + tol) + 2.0 ** -22 * ref.abs())
 
 
-def test_layer_captured_and_replayed():
-    """One graph, two sets of inputs: the replay follows the new routing with the bits of the eager run."""
+@pytest.mark.parametrize("T", [40, 700, 9000])
+def test_layer_captured_and_replayed(T):
+    """Two graphs of one layer, two sets of inputs: the replays follow the new routing with the bits of the eager run."""
     wg, wu, w_gu, w_down, sgu, sdown, router, hs = layer_weights(8, 256, 128)
-    x = randn(40, 256, seed=1, dtype=BF)
+    x = randn(T, 256, seed=1, dtype=BF)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -808,7 +809,7 @@ def test_layer_captured_and_replayed():
             out, _ = layer(x, router, w_gu, w_down, sgu, sdown, hs, 2)
         graphs.append((g, out))
     for seed in (2, 3):
-        x.copy_(randn(40, 256, seed=seed, dtype=BF))
+        x.copy_(randn(T, 256, seed=seed, dtype=BF))
         a, b = torch.cuda.Stream(), torch.cuda.Stream()
         for st, (g, _) in zip((a, b), graphs):
             st.wait_stream(torch.cuda.current_stream())

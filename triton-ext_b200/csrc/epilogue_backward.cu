@@ -40,10 +40,21 @@ __device__ __forceinline__ Piece<T, V> load_plain(const T* p) {
   }
 }
 
+template <typename T, int V>
+__device__ __forceinline__ void store_plain(T* p, const Piece<T, V>& v) {
+  if constexpr (V == 1) {
+    *p = v.e[0];
+  } else {
+    uint4 u;
+    memcpy(&u, &v, 16);
+    __stcs(reinterpret_cast<uint4*>(p), u);
+  }
+}
+
 // Grid: x = column blocks * cluster size; the CTAs of a cluster share their columns and split the rows.
 template <typename T, int V, int ACT, int TX>
 __global__ void __launch_bounds__(kEbThreads, 4) epilogue_backward_kernel(const EpiBwdParams p, int splits) {
-  constexpr int TY = kEbThreads / TX;
+  constexpr int TY = kEbThreads / TX, kUnroll = V == 1 ? 8 : kEbUnroll;
   __shared__ float part[TY][TX * V + 1];
   const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
   const int split = blockIdx.x % splits;
@@ -57,10 +68,10 @@ __global__ void __launch_bounds__(kEbThreads, 4) epilogue_backward_kernel(const 
     const T* g = reinterpret_cast<const T*>(p.grad) + c;
     const T* z = reinterpret_cast<const T*>(p.pre) + c;
     T* o = reinterpret_cast<T*>(p.out) + c;
-    for (int64_t r = r0 + ty; r < r1; r += TY * kEbUnroll) {
-      Piece<T, V> gv[kEbUnroll], zv[kEbUnroll];
+    for (int64_t r = r0 + ty; r < r1; r += TY * kUnroll) {
+      Piece<T, V> gv[kUnroll], zv[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kEbUnroll; ++u) {
+      for (int u = 0; u < kUnroll; ++u) {
         const int64_t ru = r + (int64_t)u * TY;
         if (ru < r1) {
           gv[u] = load_plain<T, V>(g + ru * p.ld_grad);
@@ -68,7 +79,7 @@ __global__ void __launch_bounds__(kEbThreads, 4) epilogue_backward_kernel(const 
         }
       }
 #pragma unroll
-      for (int u = 0; u < kEbUnroll; ++u) {
+      for (int u = 0; u < kUnroll; ++u) {
         const int64_t ru = r + (int64_t)u * TY;
         if (ru < r1) {
           Piece<T, V> ov;
@@ -95,7 +106,7 @@ __global__ void __launch_bounds__(kEbThreads, 4) epilogue_backward_kernel(const 
               }
             }
           }
-          store_piece<T, V>(o + ru * p.ld_out, ov);
+          store_plain<T, V>(o + ru * p.ld_out, ov);
         }
       }
     }

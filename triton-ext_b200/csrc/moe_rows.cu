@@ -22,13 +22,10 @@
 namespace b2x {
 
 constexpr int kRowThreads = 128;
-constexpr int kFusedPairs = 2048;   // pairs that a CTA counts by itself
-#ifndef CCTAS
-#define CCTAS 4736
-#endif
-constexpr int kCombineCtas = CCTAS;
+constexpr int kFusedPairs = 512;    // pairs that a CTA counts by itself (2048 pairs so: 19 us, in two launches 14)
 constexpr int kPlanCtas = 8;
-constexpr int kPlanThreads = 512;
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanDepth = 8;  // loads of a lane in flight
 constexpr int kPlanWarps = kPlanThreads / 32;
 
 struct DispatchParams {
@@ -45,7 +42,7 @@ struct DispatchParams {
   int32_t* offsets;
   int32_t* rows;
   int fused;  // ranks are computed here, not read from rows
-  int vec;    // x rows are 16-byte aligned, q rows too
+  int vec_x, vec_q;  // rows start on 16-byte boundaries
 };
 
 // Exclusive sums of cnt[0..E) in place by the whole CTA; cnt[E] receives the total.
@@ -63,11 +60,10 @@ __device__ __forceinline__ void block_exclusive_scan(int* cnt, int E, int* warp_
     }
     if (lane == 31) warp_part[warp] = s;
     __syncthreads();
-    int before = carry, all = carry;
-    for (int w = 0; w < warps; ++w) {
-      if (w < warp) before += warp_part[w];
-      all += warp_part[w];
-    }
+    // sums of the warps before this one and of all, the same in every warp
+    const int part = lane < warps ? warp_part[lane] : 0;
+    const int before = carry + __reduce_add_sync(0xffffffffu, lane < warp ? part : 0);
+    const int all = carry + __reduce_add_sync(0xffffffffu, part);
     if (i < E) cnt[i] = before + s - v;
     carry = all;
     __syncthreads();
@@ -77,7 +73,7 @@ __device__ __forceinline__ void block_exclusive_scan(int* cnt, int E, int* warp_
 }
 
 // One cluster sorts all pairs; see the top of the file.  Shared: hist[warps][E], then total[E + 1].
-__global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads)
+__global__ void __launch_bounds__(kPlanThreads)
     moe_plan_kernel(const int32_t* __restrict__ indices, int64_t pairs, int E, int32_t* __restrict__ offsets,
                     int32_t* __restrict__ rows) {
   extern __shared__ int plan_smem[];
@@ -85,23 +81,37 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
   int* hist = plan_smem;                 // [kPlanWarps][E]: counts, then next row of (warp, expert)
   int* total = hist + kPlanWarps * E;    // [E + 1]: this CTA's counts; peers read them
   int* start = total + E + 1;            // [E + 1]: offsets of the experts
+  int* prior = start + E + 1;            // [E]: pairs of the CTAs before this one
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t rank = cluster_ctarank();
+  const uint32_t rank = blockIdx.x, ctas = gridDim.x;  // one cluster
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the rows may be read and scaled meanwhile
   for (int i = threadIdx.x; i < kPlanWarps * E; i += kPlanThreads) hist[i] = 0;
   __syncthreads();
   // contiguous parts, a multiple of 32 pairs for each warp
-  const int64_t per_warp = ((pairs + kPlanCtas * kPlanWarps - 1) / (kPlanCtas * kPlanWarps) + 31) / 32 * 32;
+  const int64_t per_warp = ((pairs + ctas * kPlanWarps - 1) / (ctas * kPlanWarps) + 31) / 32 * 32;
   const int64_t lo = ((int64_t)rank * kPlanWarps + warp) * per_warp;
   const int64_t hi = lo + per_warp < pairs ? lo + per_warp : pairs;
   int* mine = hist + warp * E;
-  for (int64_t i = lo + lane; i - lane < hi; i += 32) {
-    const int e = i < hi ? indices[i] : -1;
-    if (e >= 0 && e < E) atomicAdd(&mine[e], 1);  // a count: the order does not matter
+  int held[kPlanDepth];  // the first pairs of the lane, for both passes; -1: dropped or none
+  for (int64_t i0 = lo; i0 < hi; i0 += 32 * kPlanDepth) {
+    int e[kPlanDepth];
+#pragma unroll
+    for (int u = 0; u < kPlanDepth; ++u) {
+      const int64_t i = i0 + 32 * u + lane;
+      e[u] = i < hi ? indices[i] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kPlanDepth; ++u) {
+      if (e[u] >= E) e[u] = -1;
+      if (i0 == lo) held[u] = e[u];
+      if (e[u] >= 0) atomicAdd(&mine[e[u]], 1);  // a count: the order does not matter
+    }
   }
   __syncthreads();
   // per expert: exclusive sums over the warps, the CTA's total
   for (int e = threadIdx.x; e < E; e += kPlanThreads) {
     int s = 0;
+#pragma unroll 8
     for (int w = 0; w < kPlanWarps; ++w) {
       const int c = hist[w * E + e];
       hist[w * E + e] = s;
@@ -111,31 +121,46 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
   }
   cluster_sync();
   for (int e = threadIdx.x; e < E; e += kPlanThreads) {
-    int before = 0, all = 0;
+    int c[kPlanCtas], before = 0, all = 0;
+#pragma unroll
     for (uint32_t r = 0; r < kPlanCtas; ++r) {
-      int c;
-      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c) : "r"(mapa_shared(smem_u32(&total[e]), r)) : "memory");
-      if (r < rank) before += c;
-      all += c;
+      c[r] = 0;
+      if (r < ctas)
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c[r]) : "r"(mapa_shared(smem_u32(&total[e]), r)) : "memory");
+    }
+#pragma unroll
+    for (uint32_t r = 0; r < kPlanCtas; ++r) {
+      if (r < rank) before += c[r];
+      all += c[r];
     }
     start[e] = all;
-    for (int w = 0; w < kPlanWarps; ++w) hist[w * E + e] += before;
+    prior[e] = before;
   }
   __syncthreads();
   block_exclusive_scan(start, E, warp_part);
   if (rank == 0)
     for (int e = threadIdx.x; e <= E; e += kPlanThreads) offsets[e] = start[e];
   // ranks, in the order of the pairs
-  for (int64_t i = lo + lane; i - lane < hi; i += 32) {
-    const int e0 = i < hi ? indices[i] : -1;
-    const int e = e0 >= 0 && e0 < E ? e0 : -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, e);
-    int row = -1;
-    if (e >= 0) row = start[e] + mine[e] + __popc(same & ((1u << lane) - 1));
-    __syncwarp();
-    if (e >= 0 && lane == 31 - __clz(same)) mine[e] += __popc(same);
-    __syncwarp();
-    if (i < hi) rows[i] = row;
+  for (int64_t i0 = lo; i0 < hi; i0 += 32 * kPlanDepth) {
+    int e[kPlanDepth];
+#pragma unroll
+    for (int u = 0; u < kPlanDepth; ++u) {
+      const int64_t i = i0 + 32 * u + lane;
+      e[u] = i0 == lo ? held[u] : (i < hi ? indices[i] : -1);
+    }
+#pragma unroll
+    for (int u = 0; u < kPlanDepth; ++u) {
+      if (i0 + 32 * u >= hi) break;
+      const int64_t i = i0 + 32 * u + lane;
+      const int ex = e[u] >= 0 && e[u] < E ? e[u] : -1;
+      const uint32_t same = __match_any_sync(0xffffffffu, ex);
+      int row = -1;
+      if (ex >= 0) row = start[ex] + prior[ex] + mine[ex] + __popc(same & ((1u << lane) - 1));
+      __syncwarp();
+      if (ex >= 0 && lane == 31 - __clz(same)) mine[ex] += __popc(same);
+      __syncwarp();
+      if (i < hi) rows[i] = row;
+    }
   }
   cluster_sync();  // peers may still read this CTA's totals
 }
@@ -149,7 +174,7 @@ template <typename T>
 __device__ __forceinline__ Raw16<T> load16(const DispatchParams& p, int64_t at, int64_t col) {
   Raw16<T> r;
   const T* s = reinterpret_cast<const T*>(p.x) + at + col;
-  if (p.vec && col + 16 <= p.cols) {
+  if (p.vec_x && col + 16 <= p.cols) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T); ++i) r.v[i] = __ldcs(reinterpret_cast<const uint4*>(s) + i);
   } else {
@@ -176,7 +201,7 @@ __device__ __forceinline__ void store16(const DispatchParams& p, const float (&v
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = quant4<FP8>(make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]), inv);
-  const bool whole = p.vec && col + 16 <= p.cols;
+  const bool whole = p.vec_q && col + 16 <= p.cols;
   for (int j = 0; j < k; ++j) {
     if (row[j] < 0) continue;
     uint8_t* q = p.q + (int64_t)row[j] * p.ld_q + col;
@@ -194,44 +219,32 @@ __device__ __forceinline__ void store16(const DispatchParams& p, const float (&v
 // longer rows, read a second time (from L2) for the cast.
 template <typename T, int NV, int FP8>
 __global__ void __launch_bounds__(kRowThreads) moe_dispatch_kernel(const DispatchParams p) {
-  extern __shared__ int row_smem[];  // fused: cnt[E + 1]; always: row[k]
+  extern __shared__ int row_smem[];  // row[k], mine[k]; fused: cnt[E + 1]
   __shared__ int warp_part[kRowThreads / 32];
   __shared__ float warp_max_[kRowThreads / 32];
   const int64_t t = blockIdx.x;
   int* row = row_smem;
-  int* cnt = row_smem + p.k;
+  int* mine = row_smem + p.k;
+  int* cnt = mine + p.k;
   const int64_t at = t * p.ld_x;
   Raw16<T> raw[NV ? NV : 1];
   float v[16];
   float amax = 0.0f;
-  // the row's loads are issued before the ranking
+  // all loads go out before anything waits for one
+  constexpr int kDepth = kFusedPairs / kRowThreads;
+  int pair_of[kDepth];  // fused: this thread's pairs
+  if (p.fused) {
+#pragma unroll
+    for (int u = 0; u < kDepth; ++u) {
+      const int64_t i = u * kRowThreads + threadIdx.x;
+      pair_of[u] = i < p.tokens * p.k ? __ldg(p.indices + i) : -1;
+    }
+    for (int j = threadIdx.x; j < p.k; j += kRowThreads) row[j] = 0, mine[j] = __ldg(p.indices + t * p.k + j);
+    for (int e = threadIdx.x; e < p.E; e += kRowThreads) cnt[e] = 0;
+  }
   if (NV) {
 #pragma unroll
     for (int n = 0; n < NV; ++n) raw[n] = load16<T>(p, at, (int64_t)(n * kRowThreads + threadIdx.x) * 16);
-  }
-  if (p.fused) {
-    const int pairs = (int)(p.tokens * p.k), own = (int)(t * p.k);
-    for (int e = threadIdx.x; e < p.E; e += kRowThreads) cnt[e] = 0;
-    for (int j = threadIdx.x; j < p.k; j += kRowThreads) row[j] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < pairs; i += kRowThreads) {
-      const int e = p.indices[i];
-      if (e >= 0 && e < p.E) atomicAdd(&cnt[e], 1);
-      for (int j = 0; j < p.k; ++j)  // pairs before this token's j-th that go to the same expert
-        if (i < own + j && e == __ldg(p.indices + own + j)) atomicAdd(&row[j], 1);
-    }
-    __syncthreads();
-    block_exclusive_scan(cnt, p.E, warp_part);
-    for (int j = threadIdx.x; j < p.k; j += kRowThreads) {
-      const int e = __ldg(p.indices + own + j);
-      const int r = e >= 0 && e < p.E ? row[j] + cnt[e] : -1;
-      row[j] = r;
-      p.rows[own + j] = r;
-    }
-    if (t == 0)
-      for (int e = threadIdx.x; e <= p.E; e += kRowThreads) p.offsets[e] = cnt[e];
-  } else {
-    for (int j = threadIdx.x; j < p.k; j += kRowThreads) row[j] = p.rows[t * p.k + j];
   }
   float s;
   if (!p.given) {
@@ -258,10 +271,35 @@ __global__ void __launch_bounds__(kRowThreads) moe_dispatch_kernel(const Dispatc
     for (int w = 0; w < kRowThreads / 32; ++w) amax = fmaxf(amax, warp_max_[w]);
     s = __fdiv_rn(amax, Fp8Traits<FP8>::kMax);
   } else {
-    __syncthreads();
     s = __ldg(p.given);
   }
   const float inv = s == 0.0f ? 0.0f : __fdiv_rn(1.0f, s);
+  if (p.fused) {
+    const int own = (int)(t * p.k);
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kDepth; ++u) {
+      const int i = u * kRowThreads + threadIdx.x, e = pair_of[u];
+      if (e >= 0 && e < p.E) atomicAdd(&cnt[e], 1);
+      if (i < own + p.k)
+        for (int j = 0; j < p.k; ++j)  // pairs before this token's j-th that go to the same expert
+          if (i < own + j && e == mine[j]) atomicAdd(&row[j], 1);
+    }
+    __syncthreads();
+    block_exclusive_scan(cnt, p.E, warp_part);
+    for (int j = threadIdx.x; j < p.k; j += kRowThreads) {
+      const int e = mine[j];
+      const int r = e >= 0 && e < p.E ? row[j] + cnt[e] : -1;
+      row[j] = r;
+      p.rows[own + j] = r;
+    }
+    if (t == 0)
+      for (int e = threadIdx.x; e <= p.E; e += kRowThreads) p.offsets[e] = cnt[e];
+  } else {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan is there
+    for (int j = threadIdx.x; j < p.k; j += kRowThreads) row[j] = p.rows[t * p.k + j];
+  }
+  __syncthreads();
   if (!p.given)
     for (int j = threadIdx.x; j < p.k; j += kRowThreads)
       if (row[j] >= 0) p.scale[row[j]] = s;
@@ -280,17 +318,29 @@ __global__ void __launch_bounds__(kRowThreads) moe_dispatch_kernel(const Dispatc
   }
 }
 
-template <typename T, int FP8>
-static void launch_dispatch_rows(const DispatchParams& p, size_t smem, cudaStream_t st) {
-  const int64_t per = (p.cols + kRowThreads * 16 - 1) / (kRowThreads * 16);
-  const unsigned grid = (unsigned)p.tokens;
-  if (per <= 1) moe_dispatch_kernel<T, 1, FP8><<<grid, kRowThreads, smem, st>>>(p);
-  else if (per <= 2) moe_dispatch_kernel<T, 2, FP8><<<grid, kRowThreads, smem, st>>>(p);
-  else if (per <= 4) moe_dispatch_kernel<T, 4, FP8><<<grid, kRowThreads, smem, st>>>(p);
-  else moe_dispatch_kernel<T, 0, FP8><<<grid, kRowThreads, smem, st>>>(p);
+template <typename T, int NV, int FP8>
+static cudaError_t launch_dispatch_t(const DispatchParams& p, size_t smem, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)p.tokens, 1, 1);
+  cfg.blockDim = dim3(kRowThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  // After a plan kernel the rows start beside it: reading and scaling x needs no plan.
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.fused ? 0 : 1;
+  return cudaLaunchKernelEx(&cfg, moe_dispatch_kernel<T, NV, FP8>, p);
 }
-
-// ---------------------------------------------------------------------------------------------------------------- combine
+template <typename T, int FP8>
+static cudaError_t launch_dispatch_rows(const DispatchParams& p, size_t smem, cudaStream_t st) {
+  const int64_t per = (p.cols + kRowThreads * 16 - 1) / (kRowThreads * 16);
+  if (per <= 1) return launch_dispatch_t<T, 1, FP8>(p, smem, st);
+  if (per <= 2) return launch_dispatch_t<T, 2, FP8>(p, smem, st);
+  if (per <= 4) return launch_dispatch_t<T, 4, FP8>(p, smem, st);
+  return launch_dispatch_t<T, 0, FP8>(p, smem, st);
+}
 
 struct CombineParams {
   const void* y;
@@ -308,10 +358,17 @@ struct CombineParams {
   float* d_weights;
 };
 
-// V consecutive values as loaded (V * sizeof(T) = 16 bytes, or one value).
+// What a thread holds of a row at a time: WIDE 16 consecutive bytes, else (rows off the 16-byte grid) four values
+// kRowThreads columns apart, so that a warp's accesses stay together.
 template <typename T, int V>
 struct Piece {
   T e[V];
+};
+template <typename T, bool WIDE>
+struct PieceOf {
+  static constexpr int V = WIDE ? 16 / (int)sizeof(T) : 4;
+  static constexpr int kStep = kRowThreads * V;  // columns of a CTA's step
+  __device__ static __forceinline__ int64_t first(int64_t step) { return step * kStep + (int64_t)threadIdx.x * (WIDE ? V : 1); }
 };
 template <typename T>
 __device__ __forceinline__ float to_f32(T v) {
@@ -331,54 +388,48 @@ __device__ __forceinline__ T from_f32(float f) {
   else
     return __float2bfloat16_rn(f);
 }
-template <typename T, int V>
-__device__ __forceinline__ Piece<T, V> load_piece(const T* p) {
-  if constexpr (V == 1) {
-    return Piece<T, V>{{*p}};
-  } else {
-    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
-    Piece<T, V> r;
-    memcpy(&r, &u, 16);
-    return r;
-  }
-}
-// The piece, or zeros where `in` is false: a predicate, not a branch, so that several loads go out together.
-template <typename T, int V>
-__device__ __forceinline__ Piece<T, V> load_piece_if(bool in, const T* p) {
-  Piece<T, V> r;
-  if constexpr (V == 1) {
-    r.e[0] = in ? *p : from_f32<T>(0.0f);
-  } else {
+// The piece at column c of a row, or zeros where `in` is false: a predicate, not a branch, so that several loads go out
+// together.
+template <typename T, bool WIDE>
+__device__ __forceinline__ Piece<T, PieceOf<T, WIDE>::V> load_piece(bool in, const T* row, int64_t c, int64_t cols) {
+  Piece<T, PieceOf<T, WIDE>::V> r;
+  if constexpr (WIDE) {
     uint4 u;
     asm volatile(
         "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
         "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
         "@q ld.global.cs.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
         : "=&r"(u.x), "=&r"(u.y), "=&r"(u.z), "=&r"(u.w)
-        : "l"(p), "r"((int)in));
+        : "l"(row + c), "r"((int)in));
     memcpy(&r, &u, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.e[i] = in && c + i * kRowThreads < cols ? row[c + i * kRowThreads] : from_f32<T>(0.0f);
   }
   return r;
 }
-template <typename T, int V>
-__device__ __forceinline__ void store_piece(T* p, const Piece<T, V>& v) {
-  if constexpr (V == 1) {
-    *p = v.e[0];
-  } else {
+template <typename T, bool WIDE>
+__device__ __forceinline__ void store_piece(T* row, int64_t c, int64_t cols, const Piece<T, PieceOf<T, WIDE>::V>& v) {
+  if constexpr (WIDE) {
     uint4 u;
     memcpy(&u, &v, 16);
-    __stcs(reinterpret_cast<uint4*>(p), u);
+    __stcs(reinterpret_cast<uint4*>(row + c), u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i * kRowThreads < cols) row[c + i * kRowThreads] = v.e[i];
   }
 }
 
-// A CTA takes a token's columns in steps of kRowThreads * V, `per` CTAs side by side.  MANY: more than 8 slots, their rows
+// A CTA takes a token's columns in steps of PieceOf::kStep, `per` CTAs side by side.  MANY: more than 8 slots, their rows
 // and weights read again for every step.
-template <typename T, int V, bool MANY>
+template <typename T, bool WIDE, bool MANY>
 __global__ void __launch_bounds__(kRowThreads) moe_combine_kernel(const CombineParams p, uint32_t per) {
+  using A = PieceOf<T, WIDE>;
   constexpr int U = 8;  // rows in flight
+  constexpr int V = A::V;
   const int64_t t = blockIdx.x / per;
   const T* y = reinterpret_cast<const T*>(p.y);
-  const int64_t step = (int64_t)per * kRowThreads * V;
   int r[U];
   float w[U];
   auto slots = [&](int j0) {
@@ -390,16 +441,18 @@ __global__ void __launch_bounds__(kRowThreads) moe_combine_kernel(const CombineP
     }
   };
   if (!MANY) slots(0);
-  for (int64_t c = ((int64_t)(blockIdx.x % per) * kRowThreads + threadIdx.x) * V; c < p.cols; c += step) {
+  const int64_t step = (int64_t)per * A::kStep;
+  for (int64_t c = A::first(blockIdx.x % per); c < p.cols; c += step) {
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-    const Piece<T, V> res = load_piece_if<T, V>(p.residual != nullptr, reinterpret_cast<const T*>(p.residual) + t * p.ld_res + c);
+    const Piece<T, V> res =
+        load_piece<T, WIDE>(p.residual != nullptr, reinterpret_cast<const T*>(p.residual) + t * p.ld_res, c, p.cols);
     for (int j0 = 0; j0 < (MANY ? p.k : 1); j0 += U) {
       if (MANY) slots(j0);
       Piece<T, V> v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = load_piece_if<T, V>(r[u] >= 0, y + (int64_t)r[u] * p.ld_y + c);
+      for (int u = 0; u < U; ++u) v[u] = load_piece<T, WIDE>(r[u] >= 0, y + (int64_t)r[u] * p.ld_y, c, p.cols);
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -408,13 +461,15 @@ __global__ void __launch_bounds__(kRowThreads) moe_combine_kernel(const CombineP
     Piece<T, V> o;
 #pragma unroll
     for (int i = 0; i < V; ++i) o.e[i] = from_f32<T>(acc[i] + to_f32(res.e[i]));
-    store_piece<T, V>(reinterpret_cast<T*>(p.out) + t * p.ld_out + c, o);
+    store_piece<T, WIDE>(reinterpret_cast<T*>(p.out) + t * p.ld_out, c, p.cols, o);
   }
 }
 
-// One CTA per token; KC slots at a time (their dot products stay in registers).
-template <typename T, int V, int KC>
+// One CTA per token; 8 slots at a time (their dot products stay in registers).
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kRowThreads) moe_combine_backward_kernel(const CombineParams p) {
+  using A = PieceOf<T, WIDE>;
+  constexpr int KC = 8, V = A::V;
   __shared__ float part[kRowThreads / 32][KC];
   const int64_t t = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -431,12 +486,11 @@ __global__ void __launch_bounds__(kRowThreads) moe_combine_backward_kernel(const
       w[u] = j0 + u < p.k ? __ldg(p.weights + t * p.k + j0 + u) : 0.0f;
       dot[u] = 0.0f;
     }
-    for (int64_t c = (int64_t)threadIdx.x * V; c < p.cols; c += kRowThreads * V) {
+    for (int64_t c = A::first(0); c < p.cols; c += A::kStep) {
       Piece<T, V> v[KC];
 #pragma unroll
-      for (int u = 0; u < KC; ++u)
-        v[u] = load_piece_if<T, V>(r[u] >= 0, y + (int64_t)r[u] * p.ld_y + c);
-      const Piece<T, V> gv = load_piece<T, V>(g + c);
+      for (int u = 0; u < KC; ++u) v[u] = load_piece<T, WIDE>(r[u] >= 0, y + (int64_t)r[u] * p.ld_y, c, p.cols);
+      const Piece<T, V> gv = load_piece<T, WIDE>(true, g, c, p.cols);
       float gf[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) gf[i] = to_f32(gv.e[i]);
@@ -449,7 +503,7 @@ __global__ void __launch_bounds__(kRowThreads) moe_combine_backward_kernel(const
           dot[u] = fmaf(gf[i], to_f32(v[u].e[i]), dot[u]);
           o.e[i] = from_f32<T>(w[u] * gf[i]);
         }
-        store_piece<T, V>(dy + (int64_t)r[u] * p.ld_out + c, o);
+        store_piece<T, WIDE>(dy + (int64_t)r[u] * p.ld_out, c, p.cols, o);
       }
     }
 #pragma unroll
@@ -469,28 +523,20 @@ __global__ void __launch_bounds__(kRowThreads) moe_combine_backward_kernel(const
   }
 }
 
-template <typename T, int BACKWARD>
-static cudaError_t launch_combine_t(const CombineParams& p, bool vec, cudaStream_t st) {
-  constexpr int V = 16 / sizeof(T);
+template <typename T, int BACKWARD, bool WIDE>
+static cudaError_t launch_combine_t(const CombineParams& p, cudaStream_t st) {
   if constexpr (BACKWARD) {
-    const unsigned grid = (unsigned)p.tokens;
-    if (vec)
-      moe_combine_backward_kernel<T, V, 8><<<grid, kRowThreads, 0, st>>>(p);
-    else
-      moe_combine_backward_kernel<T, 1, 8><<<grid, kRowThreads, 0, st>>>(p);
+    moe_combine_backward_kernel<T, WIDE><<<(unsigned)p.tokens, kRowThreads, 0, st>>>(p);
   } else {
-    const int v = vec ? V : 1;
-    // CTAs side by side on a token: all its steps while the tokens are few, fewer once they fill the GPU
-    uint32_t per = (uint32_t)((p.cols + kRowThreads * v - 1) / (kRowThreads * v));
-    while (per > 1 && p.tokens * per > kCombineCtas) per = (per + 1) / 2;
+    // CTAs side by side on a token: one a step, until there are several times more than fit the GPU at once
+    // (8191 x 7168, k = 8: 175 us with 7 CTAs a token, 180 with one; 3000 x 2049, k = 4, narrow: 63 and 43 us).
+    uint32_t per = (uint32_t)((p.cols + PieceOf<T, WIDE>::kStep - 1) / PieceOf<T, WIDE>::kStep);
+    while (per > 1 && p.tokens * per > (WIDE ? 65536 : 4736)) per = (per + 1) / 2;
     const unsigned grid = (unsigned)(p.tokens * per);
-    if (vec) {
-      p.k > 8 ? moe_combine_kernel<T, V, true><<<grid, kRowThreads, 0, st>>>(p, per)
-              : moe_combine_kernel<T, V, false><<<grid, kRowThreads, 0, st>>>(p, per);
-    } else {
-      p.k > 8 ? moe_combine_kernel<T, 1, true><<<grid, kRowThreads, 0, st>>>(p, per)
-              : moe_combine_kernel<T, 1, false><<<grid, kRowThreads, 0, st>>>(p, per);
-    }
+    if (p.k > 8)
+      moe_combine_kernel<T, WIDE, true><<<grid, kRowThreads, 0, st>>>(p, per);
+    else
+      moe_combine_kernel<T, WIDE, false><<<grid, kRowThreads, 0, st>>>(p, per);
   }
   note_launch(1);
   return cudaGetLastError();
@@ -498,9 +544,9 @@ static cudaError_t launch_combine_t(const CombineParams& p, bool vec, cudaStream
 
 template <int BACKWARD>
 static cudaError_t launch_combine(const CombineParams& p, b2x_dtype type, bool vec, cudaStream_t st) {
-  if (type == B2X_F32) return launch_combine_t<float, BACKWARD>(p, vec, st);
-  if (type == B2X_F16) return launch_combine_t<__half, BACKWARD>(p, vec, st);
-  return launch_combine_t<__nv_bfloat16, BACKWARD>(p, vec, st);
+  if (type == B2X_F32) return vec ? launch_combine_t<float, BACKWARD, true>(p, st) : launch_combine_t<float, BACKWARD, false>(p, st);
+  if (type == B2X_F16) return vec ? launch_combine_t<__half, BACKWARD, true>(p, st) : launch_combine_t<__half, BACKWARD, false>(p, st);
+  return vec ? launch_combine_t<__nv_bfloat16, BACKWARD, true>(p, st) : launch_combine_t<__nv_bfloat16, BACKWARD, false>(p, st);
 }
 
 // Rows of `elem`-byte values that start on 16-byte boundaries.
@@ -550,23 +596,37 @@ extern "C" B2X_API b2x_status b2x_moe_dispatch(const b2x_moe_dispatch_args* a, v
   p.rows = a->rows;
   const int64_t pairs = a->tokens * a->top_k;
   p.fused = pairs <= kFusedPairs;
-  p.vec = rows_aligned(a->x, a->ld_x, p.x_f32 ? 4 : 2) && rows_aligned(a->q, a->ld_q, 1);
+  p.vec_x = rows_aligned(a->x, a->ld_x, p.x_f32 ? 4 : 2);
+  p.vec_q = rows_aligned(a->q, a->ld_q, 1);
   if (!p.fused) {
-    const int smem = (kPlanWarps * p.E + 2 * (p.E + 1)) * 4;
+    const int smem = (kPlanWarps * p.E + 2 * (p.E + 1) + p.E) * 4;
     cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(moe_plan_kernel), smem);
     if (e != cudaSuccess) return cuda_fail(e, "b2x_moe_dispatch: shared memory");
-    moe_plan_kernel<<<kPlanCtas, kPlanThreads, smem, st>>>(a->indices, pairs, p.E, a->offsets, a->rows);
+    // one CTA while its warps take a few rounds of pairs, else a cluster of them
+    cudaLaunchConfig_t cfg = {};
+    const unsigned ctas = pairs <= 8 * kPlanThreads ? 1 : kPlanCtas;
+    cfg.gridDim = dim3(ctas, 1, 1);
+    cfg.blockDim = dim3(kPlanThreads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, moe_plan_kernel, a->indices, pairs, p.E, a->offsets, a->rows);
     note_launch(1);
-    e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "b2x_moe_dispatch launch (plan)");
   }
-  const size_t smem = (size_t)(p.k + (p.fused ? p.E + 1 : 0)) * 4;
+  const size_t smem = (size_t)(2 * p.k + (p.fused ? p.E + 1 : 0)) * 4;
+  cudaError_t e;
   if (p.x_f32)
-    a->q_type == B2X_E5M2 ? launch_dispatch_rows<float, 1>(p, smem, st) : launch_dispatch_rows<float, 0>(p, smem, st);
+    e = a->q_type == B2X_E5M2 ? launch_dispatch_rows<float, 1>(p, smem, st) : launch_dispatch_rows<float, 0>(p, smem, st);
   else
-    a->q_type == B2X_E5M2 ? launch_dispatch_rows<uint16_t, 1>(p, smem, st) : launch_dispatch_rows<uint16_t, 0>(p, smem, st);
+    e = a->q_type == B2X_E5M2 ? launch_dispatch_rows<uint16_t, 1>(p, smem, st) : launch_dispatch_rows<uint16_t, 0>(p, smem, st);
   note_launch(1);
-  cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? B2X_OK : cuda_fail(e, "b2x_moe_dispatch launch");
 }
 
