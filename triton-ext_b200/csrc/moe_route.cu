@@ -4,17 +4,22 @@
 // One warp owns a token; lane l holds the logits of experts VPL l .. VPL l + VPL - 1 in registers, so a row is read once
 // and a group of experts is a run of lanes.  Bound: HBM for many tokens (tokens * experts logits in), latency for few; in
 // between the instructions of the selection, so that takes few.  Choices become order-preserving 32-bit keys.  The
-// (k + 1)-th largest of the 32 lanes' maxima (redux.sync) is a bound that at least k + 1 keys reach and few more; those
+// (k + 2)-th largest of the 32 lanes' maxima (redux.sync) is a bound that at least k + 2 keys reach and few more; those
 // (almost always at most 32) are packed one to a lane in the order of their index, and each counts the better ones.  Where
 // more than 32 reach the bound the choices are taken one after the other instead.  What bounds the kernel is the integer
 // pipe, at half rate: comparisons and selections.
 //
 // What is compared.  Without a bias s is monotone in the logit, so the logits themselves are the keys and the choice is
-// exact.  With a bias (and for sums of two) the keys are fp32 values of s + b, each off by at most
-// `err` = (2^-20 + softmax: (VPL + 5) 2^-24) max s + 2^-23 max |s + b|: the approximate exponential and reciprocal together stay
-// below 2^-20 relative, the softmax's sum adds VPL + 5 roundings, and s + b is rounded once.  A row whose chosen values
-// lie closer than 2 err, or whose group scores (sums of two, 3 err each) lie closer than 6 err at the border, is chosen
-// again in fp64 (choose_exact): the choice is right to fp64, at the speed of fp32 for nearly all rows.
+// exact.  With a bias (and for sums of two) the keys are fp32 values of s + b.  s is off by at most err = 2^-20 (sigmoid) or
+// (2^-20 + (VPL + 5) 2^-24) max s: the approximate exponential and reciprocal together stay below 2^-20 relative and the
+// softmax's sum adds VPL + 5 roundings; s + b is rounded once, by 2^-24 of it.  A row in which two neighbours of the
+// order a, b lie closer than 2 err + 2^-23 (|a| + |b|), or the group scores at the border closer than twice that, is
+// settled in fp64: the groups alone (groups_exact), the candidates' order alone (rank_exact), or, where neither will do,
+// the whole choice (choose_exact).  It is right to fp64, at the speed of fp32 for nearly all rows (16384 tokens, 256
+// experts, k = 8: 34 rows needed it; settling them all by choose_exact took the kernel from 24 to 31 us).
+//
+// Measured, 16384 tokens, k = 8, 64 / 128 / 256 / 384 experts: softmax 9.8 / 10.6 / 12.2 / 13.6 us; sigmoid, bias, 8 groups by
+// their two largest 17 / 20 / 24 / 30 us.  8 tokens: 2.7 to 4.0 us, launch and latency.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
@@ -34,7 +39,7 @@ struct RouteParams {
   int type, E, k;
   int sigmoid, renorm, groups, top_groups, top2;
   int lanes_per_group;  // where a group is a run of 2^n whole lanes, else 0
-  int vec;              // rows allow 4-value loads
+  int vec, vec_b;       // logits' rows, the biases allow 4-value loads
   float scale;
   const float* bias;
   float* weights;
@@ -46,14 +51,17 @@ struct RouteParams {
   int vec_d;
 };
 
-// Unsigned order of floats: masked (-inf) 0, then rising, NaN on top; -0 and +0 are one value.
+// Unsigned order of floats: masked (-inf) 0, then rising, NaN on top; -0 and +0 are one value (the addition also makes
+// every NaN the one positive pattern).
+constexpr uint32_t kNegInf = 0x007fffffu;              // -inf with its bits turned over
+constexpr uint32_t kNaN = 0xffffffffu - kNegInf;
 __device__ __forceinline__ uint32_t order_key(float f) {
-  if (f != f) return 0xffffffffu;
   const uint32_t u = __float_as_uint(f + 0.0f);
-  return u == 0xff800000u ? 0u : (u & 0x80000000u ? ~u : u | 0x80000000u);
+  return (u ^ ((uint32_t)((int)u >> 31) | 0x80000000u)) - kNegInf;
 }
 __device__ __forceinline__ float key_value(uint32_t k) {  // of a key that is neither masked nor NaN
-  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+  const uint32_t u = k + kNegInf;
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -117,66 +125,94 @@ __device__ __forceinline__ void load_logits(const RouteParams& p, int64_t row, i
   for (int i = 0; i < VPL; ++i) l[i] = e0 + i < p.E ? load_f32(p.logits, row + e0 + i, p.type) : -INFINITY;
 }
 
-// The choice in fp64 (rows with values next to a border): lane j < k gets its expert or -1.
+// Whether the lane's group stays, from fp64 scores of its experts: groups that are runs of 2^n lanes, the two largest by
+// exchanges, the rank by counting the better groups.
 template <int VPL>
-__device__ __noinline__ int choose_exact(const RouteParams& p, int64_t row, int lane) {
-  float l[VPL];  // read again: an array handed over would live in memory for every row
-  load_logits<VPL>(p, row, lane, l);
-  double c[VPL], s[VPL];
-  bool off[VPL];
-  double m = -INFINITY, sum = 0.0;
+__device__ __forceinline__ bool keep_exact(const RouteParams& p, const double (&s)[VPL], const bool (&off)[VPL], int lane) {
+  double a1 = -INFINITY, a2 = -INFINITY;
+  int n = 0;  // how many there are, up to two
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) m = fmax(m, (double)l[i]);
+  for (int i = 0; i < VPL; ++i)
+    if (!off[i]) {
+      if (n == 0 || s[i] > a1) a2 = a1, a1 = s[i];
+      else if (n == 1 || s[i] > a2) a2 = s[i];
+      n = min(n + 1, 2);
+    }
+  for (int o = 1; o < p.lanes_per_group; o <<= 1) {
+    const double b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
+    const int bn = __shfl_xor_sync(kAll, n, o);
+    const double hi = fmax(a1, b1), lo = fmin(a1, b1);
+    a2 = fmax(lo, fmax(a2, b2));
+    a1 = hi;
+    n = min(n + bn, 2);
+  }
+  const double score = p.top2 && n == 2 ? a1 + a2 : a1;
+  const int g = lane / p.lanes_per_group;
+  int better = 0;
+  for (int i = 0; i < p.groups; ++i) {
+    const double other = __shfl_sync(kAll, score, i * p.lanes_per_group);
+    const int there = __shfl_sync(kAll, n, i * p.lanes_per_group);
+    better += there > 0 && (other > score || (other == score && i < g));
+  }
+  return n > 0 && g < p.groups && better < p.top_groups;
+}
+
+// fp64 scores of the lane's experts: s, and which of them are masked.
+template <int VPL>
+__device__ __forceinline__ void scores_exact(const RouteParams& p, const float (&l)[VPL], int e0, double (&s)[VPL], bool (&off)[VPL]) {
+  double m = 0.0, sum = 0.0;
+  if (!p.sigmoid) {
+    float top = -INFINITY;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmax(m, __shfl_xor_sync(kAll, m, o));
+    for (int i = 0; i < VPL; ++i) top = fmaxf(top, l[i]);
+    m = (double)warp_max(top);
+  }
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
     s[i] = p.sigmoid ? 1.0 / (1.0 + exp(-(double)l[i])) : exp((double)l[i] - m);
     if (l[i] == -INFINITY) s[i] = 0.0;
     sum += s[i];
   }
-  sum = warp_sum(sum);
-  const int gs = p.E / p.groups, e0 = lane * VPL;
+  if (!p.sigmoid) sum = warp_sum(sum);
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
-    const int e = e0 + i;
+    const float b = p.bias && e0 + i < p.E ? p.bias[e0 + i] : 0.0f;
     if (!p.sigmoid) s[i] /= sum;
-    const float b = p.bias && e < p.E ? p.bias[e] : 0.0f;
-    c[i] = p.bias ? s[i] + (double)b : (double)l[i];
-    s[i] += (double)b;  // what groups are scored by
-    off[i] = e >= p.E || l[i] == -INFINITY || b == -INFINITY;
-    if (c[i] != c[i]) c[i] = INFINITY;
+    s[i] += (double)b;
+    off[i] = e0 + i >= p.E || l[i] == -INFINITY || b == -INFINITY;
     if (s[i] != s[i]) s[i] = INFINITY;
   }
+}
+
+// The lane's group once more, where fp32 cannot tell the last group that stays from the first that goes.
+template <int VPL>
+__device__ __noinline__ bool groups_exact(const RouteParams& p, int64_t row, int lane) {
+  float l[VPL];
+  double s[VPL];
+  bool off[VPL];
+  load_logits<VPL>(p, row, lane, l);
+  scores_exact<VPL>(p, l, lane * VPL, s, off);
+  return keep_exact<VPL>(p, s, off, lane);
+}
+
+// The choice in fp64 (rows with values next to a border): lane j < k gets its expert or -1.
+template <int VPL>
+__device__ __noinline__ int choose_exact(const RouteParams& p, int64_t row, int lane) {
+  float l[VPL];  // read again: an array handed over would live in memory for every row
+  load_logits<VPL>(p, row, lane, l);
+  double c[VPL], s[VPL];  // what experts are chosen by; s + b, what groups are scored by
+  bool off[VPL];
+  const int gs = p.E / p.groups, e0 = lane * VPL;
+  scores_exact<VPL>(p, l, e0, s, off);
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    c[i] = p.bias ? s[i] : (double)l[i];
+    if (c[i] != c[i]) c[i] = INFINITY;
+  }
   if (p.groups > 1 && p.lanes_per_group) {
-    // runs of 2^n lanes, as in the kernel: the two largest by exchanges, the rank by counting the better groups
-    double a1 = -INFINITY, a2 = -INFINITY;
-    int n = 0;  // how many there are, up to two
+    const bool kept = keep_exact<VPL>(p, s, off, lane);
 #pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (!off[i]) {
-        if (n == 0 || s[i] > a1) a2 = a1, a1 = s[i];
-        else if (n == 1 || s[i] > a2) a2 = s[i];
-        n = min(n + 1, 2);
-      }
-    for (int o = 1; o < p.lanes_per_group; o <<= 1) {
-      const double b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
-      const int bn = __shfl_xor_sync(kAll, n, o);
-      const double hi = fmax(a1, b1), lo = fmin(a1, b1);
-      a2 = fmax(lo, fmax(a2, b2));
-      a1 = hi;
-      n = min(n + bn, 2);
-    }
-    const double score = p.top2 && n == 2 ? a1 + a2 : a1;
-    const int g = lane / p.lanes_per_group;
-    int better = 0;
-    for (int i = 0; i < p.groups; ++i) {
-      const double other = __shfl_sync(kAll, score, i * p.lanes_per_group);
-      const int there = __shfl_sync(kAll, n, i * p.lanes_per_group);
-      better += there > 0 && (other > score || (other == score && i < g));
-    }
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) off[i] = off[i] || n == 0 || better >= p.top_groups;
+    for (int i = 0; i < VPL; ++i) off[i] = off[i] || !kept;
   } else if (p.groups > 1) {
     // lane keeps the scores of the groups VPL lane .. (groups <= experts <= 32 VPL)
     double gv[VPL];
@@ -236,6 +272,39 @@ __device__ __noinline__ int choose_exact(const RouteParams& p, int64_t row, int 
   return mine;
 }
 
+// The order of the warp's candidates (lane < n: expert `at`) in fp64: the lane's rank.
+template <int VPL>
+__device__ __noinline__ int rank_exact(const RouteParams& p, int64_t row, int lane, int at, bool have) {
+  double m = 0.0, sum = 1.0;
+  if (!p.sigmoid) {
+    float l[VPL];
+    load_logits<VPL>(p, row, lane, l);
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) top = fmaxf(top, l[i]);
+    m = (double)warp_max(top);
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (l[i] != -INFINITY) sum += exp((double)l[i] - m);
+    sum = warp_sum(sum);
+  }
+  double c = -INFINITY;
+  if (have) {
+    const double x = (double)load_f32(p.logits, row + at, p.type);
+    c = (p.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - m) / sum) + (double)p.bias[at];
+    if (c != c) c = INFINITY;
+  }
+  const int n = __popc(__ballot_sync(kAll, have));
+  int better = 0;
+  for (int j = 0; j < n; ++j) {
+    const double other = __shfl_sync(kAll, c, j);
+    const int other_at = __shfl_sync(kAll, at, j);
+    better += other > c || (other == c && other_at < at);
+  }
+  return better;
+}
+
 // Largest key of the warp and the lowest index that has it (the lanes hold rising runs of indexes).
 template <int VPL>
 __device__ __forceinline__ uint32_t take_max(const uint32_t (&key)[VPL], int lane, int& at) {
@@ -251,9 +320,19 @@ __device__ __forceinline__ uint32_t take_max(const uint32_t (&key)[VPL], int lan
   return best;
 }
 
-__device__ __forceinline__ void top2_add(float& a, float& b, float v) {  // a >= b; NaN counts as the largest
-  if (!(a >= v) && a == a) b = a, a = v;
-  else if (!(b >= v) && b == b) b = v;
+// Biases of VPL consecutive experts; past the last one 0.
+template <int VPL>
+__device__ __forceinline__ void load_bias(const RouteParams& p, int e0, float (&b)[VPL]) {
+  if (VPL % 4 == 0 && p.vec_b && e0 + VPL <= p.E) {
+#pragma unroll
+    for (int i = 0; i < VPL / 4; ++i) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(p.bias + e0) + i);
+      b[4 * i] = f.x, b[4 * i + 1] = f.y, b[4 * i + 2] = f.z, b[4 * i + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) b[i] = e0 + i < p.E ? __ldg(p.bias + e0 + i) : 0.0f;
+  }
 }
 
 template <int VPL>
@@ -282,53 +361,53 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
     sum = warp_sum(sum);
     if (__any_sync(kAll, nan)) sum = NAN;
   }
-  uint32_t key[VPL];
-  float sc[VPL];  // what groups are scored by: s + b where `values`, else the logit
+  uint32_t key[VPL], gkey[VPL];  // what experts are chosen by, what groups are scored by
   float err = 0.0f;
   if (values) {
-    float hi_s = 0.0f, hi_c = 0.0f;
-    const float inv = p.sigmoid ? 0.0f : __fdiv_rn(1.0f, sum);
+    const float inv = p.sigmoid ? 0.0f : __fdiv_rn(1.0f, sum);  // also the largest s
+    err = p.sigmoid ? 0x1p-20f : (0x1p-20f + (VPL + 5) * 0x1p-24f) * inv;
+    float b[VPL];
+    if (p.bias) load_bias<VPL>(p, e0, b);
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      const float s = l[i] == -INFINITY ? 0.0f : (p.sigmoid ? sigma_fast(l[i]) : exp_approx(l[i] - m) * inv);
-      const float b = p.bias && e0 + i < p.E ? __ldg(p.bias + e0 + i) : 0.0f;
-      sc[i] = l[i] == -INFINITY || b == -INFINITY ? -INFINITY : s + b;
-      hi_s = fmaxf(hi_s, s);
-      if (fabsf(sc[i]) < INFINITY) hi_c = fmaxf(hi_c, fabsf(sc[i]));
+      const float s = p.sigmoid ? sigma_fast(l[i]) : exp_approx(l[i] - m) * inv;
+      gkey[i] = order_key(l[i] == -INFINITY || (p.bias && b[i] == -INFINITY) ? -INFINITY : (p.bias ? s + b[i] : s));
+      key[i] = p.bias ? gkey[i] : order_key(l[i]);
     }
-    err = (0x1p-20f + (p.sigmoid ? 0.0f : (VPL + 5) * 0x1p-24f)) * warp_max(hi_s) + 0x1p-23f * warp_max(hi_c);
   } else {
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) sc[i] = l[i];
+    for (int i = 0; i < VPL; ++i) gkey[i] = key[i] = order_key(l[i]);
   }
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) key[i] = order_key(p.bias ? sc[i] : l[i]);
+  auto near = [&](uint32_t a, uint32_t b, float scale) {  // a >= b, both numbers
+    const float x = key_value(a), y = key_value(b);
+    return !(x - y > scale * fmaf(0x1p-23f, fabsf(x) + fabsf(y), 2.0f * err));
+  };
   bool close = false;  // something to be told apart in fp64
   if (p.groups > 1) {
     const int gs = p.E / p.groups;
     if (p.lanes_per_group) {
       // a group is a run of 2^n lanes: its two largest by n exchanges, its rank by counting the better groups
-      float a = -INFINITY, b = -INFINITY;
+      uint32_t a = 0, b = 0;
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) top2_add(a, b, sc[i]);
+      for (int i = 0; i < VPL; ++i) b = max(b, min(a, gkey[i])), a = max(a, gkey[i]);
       for (int o = 1; o < p.lanes_per_group; o <<= 1) {
-        const float a2 = __shfl_xor_sync(kAll, a, o), b2 = __shfl_xor_sync(kAll, b, o);
-        top2_add(a, b, a2);
-        top2_add(a, b, b2);
+        const uint32_t a2 = __shfl_xor_sync(kAll, a, o);
+        if (p.top2) b = max(min(a, a2), max(b, __shfl_xor_sync(kAll, b, o)));
+        a = max(a, a2);
       }
-      if (p.top2 && b != -INFINITY) a += b;
-      const uint32_t score = order_key(a);
+      uint32_t score = a;
+      if (p.top2 && b != 0) score = a == kNaN || b == kNaN ? kNaN : order_key(key_value(a) + key_value(b));
       const int g = lane / p.lanes_per_group;
       int better = 0;
       for (int i = 0; i < p.groups; ++i) {
         const uint32_t other = __shfl_sync(kAll, score, i * p.lanes_per_group);
         better += other > score || (other == score && i < g);
       }
-      const bool kept = score != 0 && g < p.groups && better < p.top_groups;
+      bool kept = score != 0 && g < p.groups && better < p.top_groups;
       if (values) {  // the border between the groups that stay and those that go
         const uint32_t last = __reduce_min_sync(kAll, kept ? score : 0xffffffffu);
         const uint32_t next = __reduce_max_sync(kAll, !kept && g < p.groups ? score : 0u);
-        if (next != 0 && last != 0xffffffffu && next != 0xffffffffu) close = !(key_value(last) - key_value(next) > 6.0f * err);
+        if (next != 0 && last < kNaN && next < kNaN && near(last, next, 2.0f)) kept = groups_exact<VPL>(p, row, lane);
       }
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
@@ -342,7 +421,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
         const int lo = g * gs - e0, hi = lo + gs;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-          const uint32_t v = i >= lo && i < hi ? order_key(sc[i]) : 0u;
+          const uint32_t v = i >= lo && i < hi ? gkey[i] : 0u;
           b = max(b, min(a, v));
           a = max(a, v);
         }
@@ -350,7 +429,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
         if (p.top2) {
           const uint32_t who = __ballot_sync(kAll, a == score);
           const uint32_t second = __reduce_max_sync(kAll, lane == __ffs(who) - 1 ? b : a);
-          if (second != 0 && score != 0xffffffffu) score = order_key(key_value(score) + (second == 0xffffffffu ? NAN : key_value(second)));
+          if (second != 0) score = score == kNaN || second == kNaN ? kNaN : order_key(key_value(score) + key_value(second));
         }
 #pragma unroll
         for (int i = 0; i < VPL; ++i)
@@ -375,7 +454,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
       if (values && last != 0) {
         int at;
         const uint32_t next = take_max<VPL>(gk, lane, at);
-        if (next != 0 && last != 0xffffffffu && next != 0xffffffffu) close = !(key_value(last) - key_value(next) > 6.0f * err);
+        if (next != 0 && last < kNaN && next < kNaN) close = near(last, next, 2.0f);
       }
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
@@ -391,7 +470,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) top = max(top, key[i]);
-    for (int j = 0; j <= p.k; ++j) {
+    for (int j = 0; j <= p.k + 1; ++j) {
       bound = __reduce_max_sync(kAll, top);
       if (top == bound) top = 0;
     }
@@ -444,21 +523,35 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
       int e;
       const uint32_t best = take_max<VPL>(key, lane, e);
       const uint32_t last = __shfl_sync(kAll, my_key, 31);
-      if (best != 0 && last != 0xffffffffu && !(key_value(last) - key_value(best) > 2.0f * err)) close = true;
+      if (best != 0 && last < kNaN && near(last, best, 1.0f)) close = true;
     }
   }
-  int mine = lane < p.k ? at : -1;
+  bool swap = false;  // neighbours to be told apart in fp64, all among the candidates
   if (p.bias) {
     // neighbours in the order that fp32 cannot tell apart, unless logits and biases are the same: then the index decides
     const uint32_t next_key = __shfl_down_sync(kAll, my_key, 1);
     const int next_at = __shfl_down_sync(kAll, at, 1);
-    if (lane < p.k && lane < 31 && my_key != 0 && next_key != 0 && my_key != 0xffffffffu && next_key != 0xffffffffu &&
-        !(key_value(my_key) - key_value(next_key) > 2.0f * err)) {
+    if (lane < p.k && lane < 31 && my_key != 0 && next_key != 0 && my_key != kNaN && next_key != kNaN &&
+        near(my_key, next_key, 1.0f)) {
       const float la = load_f32(p.logits, row + at, p.type), lb = load_f32(p.logits, row + next_at, p.type);
-      if (!(la == lb && __ldg(p.bias + at) == __ldg(p.bias + next_at))) close = true;
+      if (!(la == lb && __ldg(p.bias + at) == __ldg(p.bias + next_at))) swap = true;
     }
   }
-  if (__any_sync(kAll, close)) mine = choose_exact<VPL>(p, row, lane);
+  close = __any_sync(kAll, close);
+  if (__any_sync(kAll, swap) && !close) {
+    const uint32_t last = __shfl_sync(kAll, my_key, p.k - 1);
+    if (n > 32 || (last != 0 && last < kNaN && near(max(last, bound), bound, 1.0f))) {
+      close = true;  // values below the bound may belong to the choice
+    } else {
+      const int better = rank_exact<VPL>(p, row, lane, at, lane < n);
+      __syncwarp();
+      if (lane < n) pack_at[warp][better] = at;
+      __syncwarp();
+      if (lane < n) at = pack_at[warp][lane];
+    }
+  }
+  int mine = lane < p.k ? at : -1;
+  if (close) mine = choose_exact<VPL>(p, row, lane);
 
   // lane j: the weight of its expert
   float w = 0.0f;
@@ -611,6 +704,7 @@ static cudaError_t launch_route(RouteParams p, cudaStream_t st) {
   }
   const int bytes = 4 * (p.type == B2X_F32 ? 4 : 2);  // of four values
   p.vec = (uintptr_t)p.logits % bytes == 0 && p.ld % 4 == 0;
+  p.vec_b = (uintptr_t)p.bias % 16 == 0;
   p.vec_d = (uintptr_t)p.d_logits % bytes == 0 && p.ld_d % 4 == 0;
   const int gs = p.E / p.groups, lanes = gs / vpl;
   p.lanes_per_group = gs % vpl == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
