@@ -370,6 +370,14 @@ typedef struct {
 B2X_API b2x_status b2x_fp8_gemm_epilogue(const b2x_gemm_args* args, const b2x_epilogue* ep, void* stream);
 
 /*
+ * Copies `rows` rows of `cols` bytes (row stride ld_src) to rows on 16-byte
+ * boundaries (dst 16-byte aligned, ld_dst % 16 == 0), with zeros up to the
+ * next multiple of 16: for fp8 operands whose rows TMA cannot address.
+ */
+B2X_API b2x_status b2x_pad_rows(const void* src, int64_t ld_src, int64_t rows, int64_t cols, void* dst, int64_t ld_dst,
+                                void* stream);
+
+/*
  * Backward of that epilogue: d_pre = grad * act'(pre) [rows, cols] of `type`
  * (bf16, fp16 or fp32; unit column strides) and, if d_bias is not NULL,
  * d_bias[n] = sum over rows of the unrounded d_pre (fp32, fixed order).  The

@@ -190,6 +190,14 @@ def test_combine_and_backward_refuse():
         refused("b2x_epilogue_backward", status, *[v if i == at else a for i, a in enumerate(ok)])
 
 
+def test_pad_rows_refuses():
+    for args, status in (((P, 10, -1, 10, P, 16), "ERR_INVALID_ARG"), ((P, 9, 4, 10, P, 16), "ERR_INVALID_ARG"),
+                         ((P, 10, 4, 10, P + 8, 16), "ERR_INVALID_ARG"), ((P, 10, 4, 10, P, 24), "ERR_INVALID_ARG"),
+                         ((None, 10, 4, 10, P, 16), "ERR_INVALID_ARG"), ((P, 20, 4, 20, P, 16), "ERR_INVALID_ARG"),
+                         ((P, 16, 1 << 40, 16, P, 16), "ERR_UNSUPPORTED")):
+        refused("b2x_pad_rows", status, *args)
+
+
 def test_python_calls_refuse_cpu_tensors():
     import b2x
     f8 = torch.zeros((4, 128)).to(torch.float8_e4m3fn)

@@ -156,6 +156,21 @@ def test_gemm_epilogue_strided_operands():
         check(b2x.gemm_epilogue(x, b, activation="relu", residual=res), y, tol)
 
 
+@pytest.mark.parametrize("rows,cols,ld,first", [(1, 1, 1, 0), (3, 15, 15, 1), (7, 33, 40, 3), (100, 257, 257, 0), (50, 1001, 1003, 2), (2, 64, 64, 5)])
+def test_pad_rows(rows, cols, ld, first):
+    """Byte for byte, zeros up to the next 16, nothing else written."""
+    import b2x
+    from b2x import _lib as L
+    src = torch.randint(0, 256, (rows * ld + 64,), device="cuda", generator=gen(1), dtype=torch.uint8)[first:]
+    pitch = -(-cols // 16) * 16 + 32
+    dst = torch.full((rows, pitch), 7, device="cuda", dtype=torch.uint8)
+    L.check(L.lib().b2x_pad_rows(src.data_ptr(), ld, rows, cols, dst.data_ptr(), pitch, torch.cuda.current_stream().cuda_stream))
+    want = torch.full_like(dst, 7)
+    want[:, :-(-cols // 16) * 16] = 0
+    want[:, :cols] = torch.as_strided(src, (rows, cols), (ld, 1))
+    assert torch.equal(dst, want)
+
+
 def test_gemm_epilogue_nan_and_inf_reach_the_output():
     import b2x
     a, b = torch.ones((4, 128), device="cuda").to(E4), torch.ones((128, 128), device="cuda").to(E4)

@@ -28,7 +28,7 @@ EXPORTED = (
     "b2x_read_device_status", "b2x_check_device", "b2x_debug_inject", "b2x_abi_version", "b2x_launch_count", "b2x_fp8_gemm_splitk_noalloc",
     "b2x_trace_read", "b2x_allreduce_signal_words", "b2x_fp8_gemm_allreduce",
     "b2x_stoch_round", "b2x_stoch_round_rs", "b2x_grouped_gemm_workspace_size", "b2x_fp8_grouped_gemm", "b2x_fp8_gemm_swiglu",
-    "b2x_fp8_gemm_epilogue", "b2x_epilogue_backward", "b2x_moe_route", "b2x_moe_route_backward", "b2x_moe_dispatch",
+    "b2x_fp8_gemm_epilogue", "b2x_pad_rows", "b2x_epilogue_backward", "b2x_moe_route", "b2x_moe_route_backward", "b2x_moe_dispatch",
     "b2x_moe_gemm", "b2x_moe_gemm_swiglu", "b2x_moe_combine", "b2x_moe_combine_backward",
 )
 
@@ -203,6 +203,7 @@ def lib() -> ctypes.CDLL:
         vp, i64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
         for name, args in {
                 "b2x_fp8_gemm_epilogue": [ctypes.POINTER(GemmArgs), ctypes.POINTER(Epilogue), vp],
+                "b2x_pad_rows": [vp, i64, i64, i64, vp, i64, vp],
                 "b2x_epilogue_backward": [vp, i64, vp, i64, vp, i64, vp, i32, i64, i64, i32, vp],
                 "b2x_moe_route": [ctypes.POINTER(MoeRouteArgs), vp],
                 "b2x_moe_route_backward": [ctypes.POINTER(MoeRouteArgs), vp, vp, i64, vp],

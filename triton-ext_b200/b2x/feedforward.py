@@ -20,7 +20,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib as L
-from .ops import FP8_DTYPES, IN_DTYPES, OUT_DTYPES, _tma_friendly
+from .ops import FP8_DTYPES, IN_DTYPES, OUT_DTYPES
 
 FLOAT_DTYPES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
@@ -113,6 +113,31 @@ def _ints(t: torch.Tensor, what: str) -> torch.Tensor:
     return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """float8 t [..., rows, cols] with 16-byte aligned rows that do not overlap: t itself or, where TMA could not address
+    it, a copy with padded rows."""
+    shape, strides = t.shape, t.stride()
+    rows, cols = shape[-2:]
+    sr, sc = strides[-2:]
+    one = len(shape) == 2 or shape[0] == 1
+    if t.data_ptr() % 16 == 0 and (sc == 1 or cols == 1) and (rows == 1 or (sr % 16 == 0 and sr >= cols)) and (
+            one or (strides[0] % 16 == 0 and strides[0] >= rows * sr)):
+        return t
+    if (sc != 1 and cols > 1) or sr < cols or not (one or strides[0] == rows * sr):
+        t = t.contiguous()
+        sr = cols
+    out = t.new_empty((*t.shape[:-1], -(-cols // 16) * 16))
+    n = t.numel() // cols if cols else 0  # rows of all experts lie one stride apart
+    _call(t.device, L.lib().b2x_pad_rows, t.data_ptr(), max(sr, cols), n, cols, out.data_ptr(), out.shape[-1])
+    return out[..., :cols]
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Row stride of an _aligned matrix; a single row may have any."""
+    rows, cols = t.shape[-2:]
+    return t.stride(-2) if rows > 1 else max(-(-cols // 16) * 16, 16)
+
+
 # ----------------------------------------------------------------------------
 # dense product with its epilogue
 
@@ -157,29 +182,20 @@ def gemm_epilogue(a: torch.Tensor, b: torch.Tensor, *, scale_a: Optional[torch.T
     if M and N:
         if K == 0:
             raise ValueError("gemm_epilogue needs K > 0")
-        if M > 1 and a.stride(0) < K:  # rows that overlap
-            a = a.contiguous()
-        sk, sn = b.stride()
-        if min(sk, sn) != 1 or max(sk, sn) < (K if sk == 1 else N):
-            b = b.contiguous()
-        a, b = _tma_friendly(a, b)
-        K = a.shape[1]
-        g, ep = L.GemmArgs(), L.Epilogue()
-        g.a, g.b, g.c = a.data_ptr(), b.data_ptr(), c.data_ptr()
-        g.M, g.N, g.K = M, N, K
-        g.lda = _ld(a)
-        sk, sn = b.stride()
-        if sk == 1 and (sn != 1 or N == 1):
-            g.ldb_k, g.ldb_n = 1, (sn if N > 1 else max(K, 16))
+        a = _aligned(a)
+        if b.stride(0) == 1 or K == 1:  # a K-major weight
+            b = _aligned(b.t())
+            ldb = (1, _pitch(b))
         else:
-            g.ldb_k, g.ldb_n = (sk if K > 1 else max(N, 16)), sn
-        g.ldc = _ld(c)
-        g.a_type, g.b_type, g.c_type = FP8_DTYPES[a.dtype], FP8_DTYPES[b.dtype], OUT_DTYPES[out_dtype]
+            b = _aligned(b)
+            ldb = (_pitch(b), 1)
+        g = L.GemmArgs(a.data_ptr(), b.data_ptr(), c.data_ptr(), M, N, K, _pitch(a), *ldb, _ld(c), FP8_DTYPES[a.dtype],
+                       FP8_DTYPES[b.dtype], OUT_DTYPES[out_dtype])
         if sa is not None:
             g.scale_mode, g.scale_a, g.scale_b = L.SCALE_TENSOR, sa.data_ptr(), sb.data_ptr()
+        ep = L.Epilogue(activation=ACTIVATIONS[activation])
         if bias is not None:
             ep.bias, ep.bias_type = bias.data_ptr(), FLOAT_DTYPES[bias.dtype]
-        ep.activation = ACTIVATIONS[activation]
         if residual is not None:
             ep.residual, ep.ld_residual = residual.data_ptr(), _ld(residual)
         if pre is not None:
@@ -212,18 +228,14 @@ def epilogue_backward(grad: torch.Tensor, pre: torch.Tensor, activation: Optiona
 # routing
 
 
-def _route_args(logits, k, score, renormalize, scale):
-    if score not in ("softmax", "sigmoid"):
-        raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
-    a = L.MoeRouteArgs()
-    a.logits, a.logits_type = logits.data_ptr(), FLOAT_DTYPES[logits.dtype]
-    a.tokens, a.experts = logits.shape
-    a.ld_logits = _ld(logits)
-    a.top_k = k
-    a.sigmoid = score == "sigmoid"
-    a.renormalize = bool(renormalize)
-    a.scale = scale
-    return a
+SCORES = {"softmax": 0, "sigmoid": 1}
+GROUP_SCORES = {"max": 0, "top2": 1}
+
+
+def _choice(table: dict, value, what: str) -> int:
+    if value not in table:
+        raise ValueError(f"{what} must be {' or '.join(map(repr, table))}, got {value!r}")
+    return table[value]
 
 
 def moe_route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Optional[torch.Tensor] = None,
@@ -239,19 +251,16 @@ def moe_route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias:
     dev = _device(logits, bias)
     if logits.dtype not in FLOAT_DTYPES:
         raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
-    logits = _matrix(logits, "logits")
-    if group_score not in ("max", "top2"):
-        raise ValueError(f"group_score must be 'max' or 'top2', got {group_score!r}")
+    logits = _rows(logits, "logits")
     T, E = logits.shape
     bias = _scale(bias, "bias", E)
-    a = _route_args(logits, top_k, score, renormalize, scale)
-    a.num_groups, a.top_groups, a.group_top2 = num_groups, top_groups, group_score == "top2"
     k = max(top_k, 0)
     weights = logits.new_empty((T, k), dtype=torch.float32)
     experts = logits.new_empty((T, k), dtype=torch.int32)
-    if bias is not None:
-        a.bias = bias.data_ptr()
-    a.weights, a.indices = weights.data_ptr(), experts.data_ptr()
+    a = L.MoeRouteArgs(logits.data_ptr(), FLOAT_DTYPES[logits.dtype], T, E, _ld(logits), top_k, _choice(SCORES, score, "score"),
+                       None if bias is None else bias.data_ptr(), num_groups, top_groups,
+                       _choice(GROUP_SCORES, group_score, "group_score"), bool(renormalize), scale, weights.data_ptr(),
+                       experts.data_ptr())
     _call(dev, L.lib().b2x_moe_route, _byref(a))
     return weights, experts
 
@@ -263,15 +272,15 @@ def moe_route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, experts
     dev = _device(logits, grad_weights, experts)
     if logits.dtype not in FLOAT_DTYPES:
         raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
-    logits = _matrix(logits, "logits")
+    logits = _rows(logits, "logits")
     T, E = logits.shape
     if experts.dim() != 2 or experts.shape[0] != T or grad_weights.shape != experts.shape:
         raise ValueError(f"experts {tuple(experts.shape)} and grad_weights {tuple(grad_weights.shape)} must be [{T}, top_k]")
     experts = _ints(experts, "experts")
     d = grad_weights if grad_weights.dtype == torch.float32 and grad_weights.is_contiguous() else grad_weights.to(torch.float32).contiguous()
     out = logits.new_empty((T, E))
-    a = _route_args(logits, experts.shape[1], score, renormalize, scale)
-    a.indices = experts.data_ptr()
+    a = L.MoeRouteArgs(logits.data_ptr(), FLOAT_DTYPES[logits.dtype], T, E, _ld(logits), experts.shape[1],
+                       _choice(SCORES, score, "score"), None, 1, 1, 0, bool(renormalize), scale, None, experts.data_ptr())
     _call(dev, L.lib().b2x_moe_route_backward, _byref(a), d.data_ptr(), out.data_ptr(), E)
     return out
 
@@ -304,15 +313,9 @@ def moe_dispatch(x: torch.Tensor, experts: torch.Tensor, num_experts: int, *, dt
     scales = x.new_empty(T * k, dtype=torch.float32) if given is None else given
     offsets = x.new_empty(max(num_experts, 0) + 1, dtype=torch.int32)
     rows = x.new_empty((T, k), dtype=torch.int32)
-    a = L.MoeDispatchArgs()
-    a.x, a.x_type, a.tokens, a.cols, a.ld_x = x.data_ptr(), IN_DTYPES[x.dtype], T, H, _ld(x)
-    a.indices, a.top_k, a.experts = experts.data_ptr(), k, num_experts
-    a.q, a.q_type, a.ld_q = q.data_ptr(), FP8_DTYPES[dtype], _ld(q)
-    if given is None:
-        a.scale = scales.data_ptr()
-    else:
-        a.given = given.data_ptr()
-    a.offsets, a.rows = offsets.data_ptr(), rows.data_ptr()
+    a = L.MoeDispatchArgs(x.data_ptr(), IN_DTYPES[x.dtype], T, H, _ld(x), experts.data_ptr(), k, num_experts, q.data_ptr(),
+                          FP8_DTYPES[dtype], _ld(q), scales.data_ptr() if given is None else None,
+                          None if given is None else given.data_ptr(), offsets.data_ptr(), rows.data_ptr())
     _call(dev, L.lib().b2x_moe_dispatch, _byref(a))
     return q, scales, MoePlan(offsets, rows)
 
@@ -374,19 +377,6 @@ def moe_combine_backward(grad: torch.Tensor, y: torch.Tensor, rows: torch.Tensor
 # the experts' products
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """t [..., rows, cols] with unit column stride, 16-byte aligned rows and base: t itself, or a padded copy."""
-    ok = t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and t.stride(-2) % 16 == 0 and t.stride(-2) >= t.shape[-1]
-    if ok and t.dim() == 3:
-        ok = t.shape[0] == 1 or (t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1] * t.stride(1))
-    if ok:
-        return t
-    n = t.shape[-1]
-    out = torch.zeros((*t.shape[:-1], -(-n // 16) * 16), dtype=t.dtype, device=t.device)
-    out[..., :n] = t
-    return out[..., :n]
-
-
 def _moe_gemm_args(x, w, offsets, scale_x, scale_w, who, kmajor):
     if x.dtype not in FP8_DTYPES or w.dtype not in FP8_DTYPES:
         raise TypeError(f"{who} takes float8 x and w, got {x.dtype} and {w.dtype}")
@@ -399,20 +389,17 @@ def _moe_gemm_args(x, w, offsets, scale_x, scale_w, who, kmajor):
         raise ValueError(f"{who} needs K > 0")
     offsets = _ints(offsets, "offsets")
     x = _aligned(x)
-    if w.stride(2) != 1 and w.stride(1) == 1 and not kmajor:
-        w = _aligned(w.transpose(1, 2)).transpose(1, 2)  # row-major [K, N]
+    if w.stride(2) != 1 and w.stride(1) == 1 and not kmajor:  # a transposed view of [E, K, N]
+        w = _aligned(w.transpose(1, 2))
+        ldw = (w.stride(0), 1, _pitch(w))
     else:
         w = _aligned(w)
+        ldw = (w.stride(0), _pitch(w), 1)
     sx, sw = _scale(scale_x, "scale_x", 1, x.shape[0]), _scale(scale_w, "scale_w", 1, E)
-    a = L.MoeGemmArgs()
-    a.x, a.x_type, a.rows, a.K, a.ld_x = x.data_ptr(), FP8_DTYPES[x.dtype], x.shape[0], K, max(x.stride(0), K + -K % 16)
-    a.w, a.w_type, a.experts, a.N = w.data_ptr(), FP8_DTYPES[w.dtype], E, N
-    a.ldw_e, a.ldw_n, a.ldw_k = w.stride()
-    a.offsets = offsets.data_ptr()
-    if sx is not None:
-        a.scale_x, a.scale_x_count = sx.data_ptr(), sx.numel()
-    if sw is not None:
-        a.scale_w, a.scale_w_count = sw.data_ptr(), sw.numel()
+    R = x.shape[0]
+    a = L.MoeGemmArgs(x.data_ptr(), FP8_DTYPES[x.dtype], R, K, _pitch(x), w.data_ptr(), FP8_DTYPES[w.dtype],
+                      E, N, *ldw, offsets.data_ptr(), None if sx is None else sx.data_ptr(), 0 if sx is None else sx.numel(),
+                      None if sw is None else sw.data_ptr(), 0 if sw is None else sw.numel())
     return a, (x, w, offsets, sx, sw)
 
 

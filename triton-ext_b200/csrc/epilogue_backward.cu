@@ -3,7 +3,8 @@
 // One pass: a thread owns one 16-byte run of columns (V values) and walks down rows, TX threads side by side and the
 // rest of the CTA below one another; column sums stay in fp32 registers, meet in shared memory within the CTA and over
 // distributed shared memory within a cluster of up to 8 CTAs that splits the rows.  Every sum has a fixed order, there
-// is no workspace and no atomic.  Bound: HBM, three times the matrix.
+// is no workspace and no atomic.  Bound: HBM, three times the matrix (4000 x 28672 bf16 without an activation: 89 us),
+// and with an activation the instructions of its slope (gelu_tanh 126 us, gelu 158 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
