@@ -3,8 +3,10 @@
 // One pass: a thread owns one 16-byte run of columns (V values) and walks down rows, TX threads side by side and the
 // rest of the CTA below one another; column sums stay in fp32 registers, meet in shared memory within the CTA and over
 // distributed shared memory within a cluster of up to 8 CTAs that splits the rows.  Every sum has a fixed order, there
-// is no workspace and no atomic.  Bound: HBM, three times the matrix (4000 x 28672 bf16 without an activation: 89 us),
-// and with an activation the instructions of its slope (gelu_tanh 126 us, gelu 158 us).
+// is no workspace and no atomic.  The rows come through a ring in shared memory that each thread fills for itself ahead
+// (cp.async): loads into registers left too few bytes on the way beside the slope's own registers.
+// Bound: HBM, three times the matrix, and the instructions of the slope: 4000 x 28672 bf16 gelu_tanh 120 us (5.7 TB/s; with
+// loads into registers 126, with single fp32 operations besides 248), gelu 147 us; 8192 x 1024 silu 12 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
@@ -15,7 +17,8 @@
 namespace b2x {
 
 constexpr int kEbThreads = 256;
-constexpr int kEbUnroll = 2;  // rows in flight per thread (1 to 4 with 2 to 6 CTAs per SM: 126 us here, 145 to 275 elsewhere)
+constexpr int kEbUnroll = 2;  // rows of a stage
+constexpr int kEbStages = 3;  // stages of the ring: 128 KB on the way per SM beside the one that is worked on
 
 struct EpiBwdParams {
   const void* grad;
@@ -28,35 +31,19 @@ struct EpiBwdParams {
   int64_t rows, cols;
 };
 
-// Plain loads: d_pre may be grad or pre.
-template <typename T, int V>
-__device__ __forceinline__ Piece<T, V> load_plain(const T* p) {
-  if constexpr (V == 1) {
-    return Piece<T, V>{{*p}};
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    Piece<T, V> r;
-    memcpy(&r, &u, 16);
-    return r;
-  }
-}
-
-template <typename T, int V>
-__device__ __forceinline__ void store_plain(T* p, const Piece<T, V>& v) {
-  if constexpr (V == 1) {
-    *p = v.e[0];
-  } else {
-    uint4 u;
-    memcpy(&u, &v, 16);
-    __stcs(reinterpret_cast<uint4*>(p), u);
-  }
+// 16 bytes from global to shared memory, past L1 (d_pre may be grad or pre: a thread reads its values before it writes
+// them, and no other thread touches them).
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 // Grid: x = column blocks * cluster size; the CTAs of a cluster share their columns and split the rows.
 template <typename T, int V, int ACT, int TX>
 __global__ void __launch_bounds__(kEbThreads, 4) epilogue_backward_kernel(const EpiBwdParams p, int splits) {
-  constexpr int TY = kEbThreads / TX, kUnroll = V == 1 ? 8 : kEbUnroll;
-  __shared__ float part[TY][TX * V + 1];
+  constexpr int TY = kEbThreads / TX, U = kEbUnroll;
+  // [stage][g and z of U rows][thread] on the way, and at the end the column sums [TY][TX * V + 1]
+  extern __shared__ __align__(16) uint8_t eb_smem[];
+  float (*part)[TX * V + 1] = reinterpret_cast<float (*)[TX * V + 1]>(eb_smem);
   const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
   const int split = blockIdx.x % splits;
   const int64_t c = ((int64_t)(blockIdx.x / splits) * TX + tx) * V;
@@ -69,49 +56,83 @@ __global__ void __launch_bounds__(kEbThreads, 4) epilogue_backward_kernel(const 
     const T* g = reinterpret_cast<const T*>(p.grad) + c;
     const T* z = reinterpret_cast<const T*>(p.pre) + c;
     T* o = reinterpret_cast<T*>(p.out) + c;
-    for (int64_t r = r0 + ty; r < r1; r += TY * kUnroll) {
-      Piece<T, V> gv[kUnroll], zv[kUnroll];
+    if constexpr (V == 1) {
+      constexpr int kRows = 8;  // in flight
+      for (int64_t r = r0 + ty; r < r1; r += TY * kRows) {
+        T gv[kRows], zv[kRows];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int64_t ru = r + (int64_t)u * TY;
-        if (ru < r1) {
-          gv[u] = load_plain<T, V>(g + ru * p.ld_grad);
-          zv[u] = load_plain<T, V>(z + ru * p.ld_pre);
+        for (int u = 0; u < kRows; ++u) {
+          const int64_t ru = r + (int64_t)u * TY;
+          if (ru < r1) gv[u] = g[ru * p.ld_grad], zv[u] = ACT != B2X_ACT_NONE ? z[ru * p.ld_pre] : gv[u];
+        }
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+          const int64_t ru = r + (int64_t)u * TY;
+          if (ru < r1) {
+            float d, none;
+            unpair(act_slope<ACT>(pair(to_f32(zv[u]))), d, none);
+            d *= to_f32(gv[u]);
+            sum[0] += d;
+            o[ru * p.ld_out] = from_f32<T>(d);
+          }
         }
       }
+    } else {
+      // A thread copies its own pieces ahead (cp.async) and reads them back itself: no barrier.
+      const uint32_t ring = smem_u32(eb_smem) + threadIdx.x * 16;
+      auto slot = [&](int stage, int k) { return ring + (stage * 2 * U + k) * kEbThreads * 16; };
+      auto fetch = [&](int64_t r, int stage) {
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int64_t ru = r + (int64_t)u * TY;
-        if (ru < r1) {
-          Piece<T, V> ov;
-          if constexpr (V == 1) {
-            float d, none;
-            unpair(act_slope<ACT>(pair(to_f32(zv[u].e[0]))), d, none);
-            d *= to_f32(gv[u].e[0]);
-            sum[0] += d;
-            ov.e[0] = from_f32<T>(d);
-          } else {
+        for (int u = 0; u < U; ++u) {
+          const int64_t ru = r + (int64_t)u * TY;
+          if (ru < r1) {
+            copy_async16(slot(stage, 2 * u), g + ru * p.ld_grad);
+            if (ACT != B2X_ACT_NONE) copy_async16(slot(stage, 2 * u + 1), z + ru * p.ld_pre);
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      int64_t ahead = r0 + ty;
 #pragma unroll
-            for (int i = 0; i < V; i += 2) {
-              const Pair z2 = pair(to_f32(zv[u].e[i]), to_f32(zv[u].e[i + 1]));
-              const Pair d2 = mul2(pair(to_f32(gv[u].e[i]), to_f32(gv[u].e[i + 1])), act_slope<ACT>(z2));
-              float a, b;
-              unpair(add2(pair(sum[i], sum[i + 1]), d2), sum[i], sum[i + 1]);
-              unpair(d2, a, b);
-              if constexpr (__is_same(T, __nv_bfloat16)) {
-                const uint32_t w = pack_bf16x2(a, b);
-                memcpy(&ov.e[i], &w, 4);
-              } else {
-                ov.e[i] = from_f32<T>(a);
-                ov.e[i + 1] = from_f32<T>(b);
-              }
+      for (int s = 0; s < kEbStages - 1; ++s, ahead += TY * U) fetch(ahead, s);
+      int stage = 0;
+      for (int64_t r = r0 + ty; r < r1; r += TY * U, ahead += TY * U) {
+        fetch(ahead, stage == 0 ? kEbStages - 1 : stage - 1);  // the stage that was read last
+        asm volatile("cp.async.wait_group %0;" ::"n"(kEbStages - 1) : "memory");
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t ru = r + (int64_t)u * TY;
+          if (ru >= r1) continue;
+          const uint4 gw = ld_shared_u32x4(slot(stage, 2 * u));
+          const uint4 zw = ACT != B2X_ACT_NONE ? ld_shared_u32x4(slot(stage, 2 * u + 1)) : gw;  // the slope 1 needs none
+          Piece<T, V> gv, zv, ov;
+          memcpy(&gv, &gw, 16);
+          memcpy(&zv, &zw, 16);
+#pragma unroll
+          for (int i = 0; i < V; i += 2) {
+            const Pair z2 = pair(to_f32(zv.e[i]), to_f32(zv.e[i + 1]));
+            const Pair d2 = mul2(pair(to_f32(gv.e[i]), to_f32(gv.e[i + 1])), act_slope<ACT>(z2));
+            float a, b;
+            unpair(add2(pair(sum[i], sum[i + 1]), d2), sum[i], sum[i + 1]);
+            unpair(d2, a, b);
+            if constexpr (__is_same(T, __nv_bfloat16)) {
+              const uint32_t w = pack_bf16x2(a, b);
+              memcpy(&ov.e[i], &w, 4);
+            } else {
+              ov.e[i] = from_f32<T>(a);
+              ov.e[i + 1] = from_f32<T>(b);
             }
           }
-          store_plain<T, V>(o + ru * p.ld_out, ov);
+          uint4 w;
+          memcpy(&w, &ov, 16);
+          __stcs(reinterpret_cast<uint4*>(o + ru * p.ld_out), w);
         }
+        stage = stage + 1 == kEbStages ? 0 : stage + 1;
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
   }
+  __syncthreads();  // the ring is done with
   if (!p.d_bias) return;  // uniform over the grid
 #pragma unroll
   for (int i = 0; i < V; ++i) part[ty][tx * V + i] = sum[i];
@@ -154,6 +175,9 @@ static cudaError_t launch_epi_bwd_t(const EpiBwdParams& p, int num_sms, cudaStre
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(blocks * splits), 1, 1);
   cfg.blockDim = dim3(kEbThreads, 1, 1);
+  constexpr int kSums = kEbThreads / TX * (TX * V + 1) * 4, kRing = V == 1 ? 0 : kEbStages * 2 * kEbUnroll * kEbThreads * 16;
+  static_assert(kRing <= 48 << 10 && kSums <= 48 << 10, "shared memory without opting in");
+  cfg.dynamicSmemBytes = kRing > kSums ? kRing : kSums;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
