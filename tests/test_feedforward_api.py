@@ -249,3 +249,10 @@ def test_python_calls_refuse_bad_arguments():
             f()
             print("not refused:", n)
     torch.cuda.synchronize()
+
+
+def test_indices_past_int32_do_not_wrap():
+    """An int64 index outside int32 stays out of range (dropped) instead of becoming another one."""
+    from b2x.feedforward import _ints
+    t = torch.tensor([[1 << 32, 3], [-(1 << 32) + 1, (1 << 31) + 2], [-1, 0]])
+    assert _ints(t, "experts").tolist() == [[(1 << 31) - 1, 3], [-1, (1 << 31) - 1], [-1, 0]]

@@ -110,7 +110,9 @@ def _scale(t: Optional[torch.Tensor], what: str, *counts: int) -> Optional[torch
 def _ints(t: torch.Tensor, what: str) -> torch.Tensor:
     if t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
-    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    if t.dtype is torch.int64:
+        t = t.clamp(-1, 2**31 - 1).to(torch.int32)  # what int32 cannot hold stays out of range instead of wrapping
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -356,7 +358,8 @@ def moe_combine(y: torch.Tensor, rows: torch.Tensor, weights: Optional[torch.Ten
 def moe_combine_backward(grad: torch.Tensor, y: torch.Tensor, rows: torch.Tensor, weights: torch.Tensor, *,
                          out: Optional[torch.Tensor] = None):
     """(d_y [R, H], d_weights fp32 [T, top_k]) of moe_combine for grad [T, H] of y's dtype.  The residual's gradient is
-    grad.  Rows of d_y that no pair names are not written (d_y may be given as `out`)."""
+    grad.  No row may be named by two pairs, as in a plan of moe_dispatch.  Rows of d_y that no pair names are not written
+    (d_y may be given as `out`)."""
     dev = _device(y, grad, rows, weights, out)
     if y.dtype not in FLOAT_DTYPES or grad.dtype != y.dtype:
         raise TypeError(f"y and grad must both be float32, bfloat16 or float16, got {y.dtype} and {grad.dtype}")
