@@ -256,3 +256,22 @@ def test_indices_past_int32_do_not_wrap():
     from b2x.feedforward import _ints
     t = torch.tensor([[1 << 32, 3], [-(1 << 32) + 1, (1 << 31) + 2], [-1, 0]])
     assert _ints(t, "experts").tolist() == [[(1 << 31) - 1, 3], [-1, (1 << 31) - 1], [-1, 0]]
+
+
+def test_values_off_their_own_grid_are_refused():
+    """A pointer that is no multiple of its element's size would be a misaligned access."""
+    refused("b2x_fp8_gemm_epilogue", "ERR_INVALID_ARG", gemm(), epi(residual=P + 1, ld_residual=256))
+    refused("b2x_fp8_gemm_epilogue", "ERR_INVALID_ARG", gemm(), epi(pre=P + 1, ld_pre=256))
+    refused("b2x_fp8_gemm_epilogue", "ERR_INVALID_ARG", gemm(), epi(bias=P + 2, bias_type=0))
+    refused("b2x_fp8_gemm_epilogue", "ERR_INVALID_ARG", gemm(), epi(bias=P + 1, bias_type=1))
+    refused("b2x_moe_route", "ERR_INVALID_ARG", route(logits=P + 2))
+    refused("b2x_moe_dispatch", "ERR_INVALID_ARG", dispatch(x=P + 1))
+    ok = [P, 8, 64, P, P, 4, 2, 64, P, 64, P, 64, 0]
+    for at in (0, 8, 10):
+        refused("b2x_moe_combine", "ERR_INVALID_ARG", *[P + 2 if i == at else a for i, a in enumerate(ok)])
+    ok = [P, 64, P, 8, 64, P, P, 4, 2, 64, P, 64, P, 0]
+    for at in (0, 2, 10):
+        refused("b2x_moe_combine_backward", "ERR_INVALID_ARG", *[P + 2 if i == at else a for i, a in enumerate(ok)])
+    ok = [P, 64, P, 64, P, 64, P, 0, 4, 64, 0]
+    for at in (0, 2, 4):
+        refused("b2x_epilogue_backward", "ERR_INVALID_ARG", *[P + 2 if i == at else a for i, a in enumerate(ok)])

@@ -235,8 +235,10 @@ extern "C" B2X_API b2x_status b2x_epilogue_backward(const void* grad, int64_t ld
     return e == cudaSuccess ? B2X_OK : cuda_fail(e, "b2x_epilogue_backward: clearing d_bias");
   }
   if (!grad || !pre || !d_pre) return fail(B2X_ERR_INVALID_ARG, "b2x_epilogue_backward: NULL pointer");
-  EpiBwdParams p{grad, ld_grad, pre, ld_pre, d_pre, ld_d_pre, d_bias, rows, cols};
   const int elem = type == B2X_F32 ? 4 : 2;
+  if (off_grid(grad, elem) || off_grid(pre, elem) || off_grid(d_pre, elem) || off_grid(d_bias, 4))
+    return fail(B2X_ERR_INVALID_ARG, "b2x_epilogue_backward: misaligned pointer");
+  EpiBwdParams p{grad, ld_grad, pre, ld_pre, d_pre, ld_d_pre, d_bias, rows, cols};
   const bool vec = cols % (16 / elem) == 0 && rows_aligned(grad, ld_grad, elem) && rows_aligned(pre, ld_pre, elem) &&
                    rows_aligned(d_pre, ld_d_pre, elem);
   int dev = 0;

@@ -842,6 +842,8 @@ static b2x_status moe_gemm_params(const b2x_moe_gemm_args* a, const char* who, b
   if ((a->scale_x && a->scale_x_count != 1 && a->scale_x_count != a->rows) ||
       (a->scale_w && a->scale_w_count != 1 && a->scale_w_count != a->experts))
     return fail(B2X_ERR_INVALID_ARG, "%s: scale_x has one element or one per row, scale_w one or one per expert", who);
+  if (off_grid(a->offsets, 4) || off_grid(a->scale_x, 4) || off_grid(a->scale_w, 4))
+    return fail(B2X_ERR_INVALID_ARG, "%s: misaligned pointer", who);
   if (swiglu) {
     if (g.w_kind != 0) return fail(B2X_ERR_UNSUPPORTED, "%s: w must be K-major", who);
     if (a->N % 256) return fail(B2X_ERR_UNSUPPORTED, "%s: N (gate + up rows) must be a multiple of 256", who);
@@ -901,6 +903,7 @@ extern "C" B2X_API b2x_status b2x_moe_gemm_swiglu(const b2x_moe_gemm_args* a, vo
   if (!h || ld_h < a->N / 2 || ld_h % 16 || (uintptr_t)h % 16)
     return fail(B2X_ERR_INVALID_ARG, "b2x_moe_gemm_swiglu: h must be 16-byte aligned with ld_h >= N/2 and ld_h %% 16 == 0");
   if (!h_scale) return fail(B2X_ERR_INVALID_ARG, "b2x_moe_gemm_swiglu: NULL h_scale");
+  if (off_grid(h_scale, 4) || off_grid(h_amax, 4)) return fail(B2X_ERR_INVALID_ARG, "b2x_moe_gemm_swiglu: misaligned pointer");
   g.p.h = reinterpret_cast<uint8_t*>(h);
   g.p.ld_h = ld_h;
   g.p.h_e5m2 = h_type == B2X_E5M2;
@@ -947,6 +950,9 @@ extern "C" B2X_API b2x_status b2x_fp8_gemm_epilogue(const b2x_gemm_args* a, cons
     return fail(B2X_ERR_INVALID_ARG, "b2x_fp8_gemm_epilogue: B needs 16-byte alignment and a row stride %% 16 == 0");
   if (a->ldc < a->N || (uintptr_t)a->c % 2 || (ep->residual && ep->ld_residual < a->N) || (ep->pre && ep->ld_pre < a->N))
     return fail(B2X_ERR_INVALID_ARG, "b2x_fp8_gemm_epilogue: row strides of C, residual and pre must be >= N");
+  if (off_grid(ep->residual, 2) || off_grid(ep->pre, 2) || off_grid(ep->bias, ep->bias_type == B2X_F32 ? 4 : 2) ||
+      (a->scale_mode != B2X_SCALE_NONE && (off_grid(a->scale_a, 4) || off_grid(a->scale_b, 4))))
+    return fail(B2X_ERR_INVALID_ARG, "b2x_fp8_gemm_epilogue: misaligned pointer");
   b2x_status s;
   g.num_sms = b2x_device_sms("b2x_fp8_gemm_epilogue", s);
   if (s != B2X_OK) return s;

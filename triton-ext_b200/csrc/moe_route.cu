@@ -731,6 +731,9 @@ static cudaError_t launch_route(RouteParams p, cudaStream_t st) {
   return cudaGetLastError();
 }
 
+// Values of `bytes` each that do not start on a multiple of it: a misaligned access.
+static bool off_grid(const void* p, int bytes) { return (uintptr_t)p % bytes != 0; }
+
 static b2x_status route_params(const b2x_moe_route_args* a, const char* who, bool backward, RouteParams& p) {
   if (!a) return fail(B2X_ERR_INVALID_ARG, "%s: args is NULL", who);
   if (a->logits_type != B2X_F32 && a->logits_type != B2X_BF16 && a->logits_type != B2X_F16)
@@ -749,6 +752,9 @@ static b2x_status route_params(const b2x_moe_route_args* a, const char* who, boo
                 a->num_groups, a->top_groups);
   if (a->tokens > 0 && (!a->logits || !a->indices || (!backward && !a->weights)))
     return fail(B2X_ERR_INVALID_ARG, "%s: NULL pointer", who);
+  if (off_grid(a->logits, a->logits_type == B2X_F32 ? 4 : 2) || off_grid(a->bias, 4) || off_grid(a->weights, 4) ||
+      off_grid(a->indices, 4))
+    return fail(B2X_ERR_INVALID_ARG, "%s: misaligned pointer", who);
   p.logits = a->logits;
   p.ld = a->ld_logits;
   p.tokens = a->tokens;
@@ -789,6 +795,8 @@ extern "C" B2X_API b2x_status b2x_moe_route_backward(const b2x_moe_route_args* a
   if (ld_d_logits < p.E) return fail(B2X_ERR_INVALID_ARG, "b2x_moe_route_backward: ld_d_logits < experts");
   if (p.tokens == 0) return B2X_OK;
   if (!d_weights || !d_logits) return fail(B2X_ERR_INVALID_ARG, "b2x_moe_route_backward: NULL pointer");
+  if (off_grid(d_weights, 4) || off_grid(d_logits, args->logits_type == B2X_F32 ? 4 : 2))
+    return fail(B2X_ERR_INVALID_ARG, "b2x_moe_route_backward: misaligned pointer");
   p.d_weights = d_weights;
   p.d_logits = d_logits;
   p.ld_d = ld_d_logits;

@@ -574,6 +574,9 @@ extern "C" B2X_API b2x_status b2x_moe_dispatch(const b2x_moe_dispatch_args* a, v
     return fail(B2X_ERR_UNSUPPORTED, "b2x_moe_dispatch: at most 1024 experts and top_k 1024");
   if (a->tokens * a->top_k >= (1LL << 31)) return fail(B2X_ERR_UNSUPPORTED, "b2x_moe_dispatch: tokens * top_k must be < 2^31");
   if (!a->offsets) return fail(B2X_ERR_INVALID_ARG, "b2x_moe_dispatch: NULL offsets");
+  if (off_grid(a->x, a->x_type == B2X_F32 ? 4 : 2) || off_grid(a->indices, 4) || off_grid(a->scale, 4) || off_grid(a->given, 4) ||
+      off_grid(a->offsets, 4) || off_grid(a->rows, 4))
+    return fail(B2X_ERR_INVALID_ARG, "b2x_moe_dispatch: misaligned pointer");
   cudaStream_t st = (cudaStream_t)stream;
   if (a->tokens == 0) {
     cudaError_t e = cudaMemsetAsync(a->offsets, 0, (size_t)(a->experts + 1) * 4, st);
@@ -643,6 +646,9 @@ extern "C" B2X_API b2x_status b2x_moe_combine(const void* y, int64_t y_rows, int
     return fail(B2X_ERR_INVALID_ARG, "b2x_moe_combine: bad shape or row stride");
   if (tokens == 0 || cols == 0) return B2X_OK;
   if ((y_rows > 0 && !y) || !rows || !out) return fail(B2X_ERR_INVALID_ARG, "b2x_moe_combine: NULL pointer");
+  const int elem = type == B2X_F32 ? 4 : 2;
+  if (off_grid(y, elem) || off_grid(residual, elem) || off_grid(out, elem) || off_grid(rows, 4) || off_grid(weights, 4))
+    return fail(B2X_ERR_INVALID_ARG, "b2x_moe_combine: misaligned pointer");
   CombineParams p{};
   p.y = y;
   p.y_rows = y_rows;
@@ -656,7 +662,6 @@ extern "C" B2X_API b2x_status b2x_moe_combine(const void* y, int64_t y_rows, int
   p.ld_res = ld_residual;
   p.out = out;
   p.ld_out = ld_out;
-  const int elem = type == B2X_F32 ? 4 : 2;
   const bool vec = cols % (16 / elem) == 0 && rows_aligned(y, ld_y, elem) && rows_aligned(out, ld_out, elem) &&
                    (!residual || rows_aligned(residual, ld_residual, elem));
   const int64_t ctas = tokens * ((cols + kRowThreads - 1) / kRowThreads);
@@ -678,6 +683,9 @@ extern "C" B2X_API b2x_status b2x_moe_combine_backward(const void* grad, int64_t
   if (tokens == 0) return B2X_OK;
   if (!rows || !weights || !d_weights || (cols > 0 && (!grad || (y_rows > 0 && (!y || !d_y)))))
     return fail(B2X_ERR_INVALID_ARG, "b2x_moe_combine_backward: NULL pointer");
+  const int elem = type == B2X_F32 ? 4 : 2;
+  if (off_grid(grad, elem) || off_grid(y, elem) || off_grid(d_y, elem) || off_grid(rows, 4) || off_grid(weights, 4) || off_grid(d_weights, 4))
+    return fail(B2X_ERR_INVALID_ARG, "b2x_moe_combine_backward: misaligned pointer");
   CombineParams p{};
   p.y = y;
   p.y_rows = y_rows;
@@ -692,7 +700,6 @@ extern "C" B2X_API b2x_status b2x_moe_combine_backward(const void* grad, int64_t
   p.grad = grad;
   p.ld_grad = ld_grad;
   p.d_weights = d_weights;
-  const int elem = type == B2X_F32 ? 4 : 2;
   const bool vec = cols % (16 / elem) == 0 && rows_aligned(y, ld_y, elem) && rows_aligned(d_y, ld_d_y, elem) &&
                    rows_aligned(grad, ld_grad, elem);
   cudaError_t e = launch_combine<1>(p, type, vec, (cudaStream_t)stream);
