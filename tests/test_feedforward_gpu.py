@@ -225,6 +225,36 @@ def test_epilogue_backward_against_differences(name):
     check(d, ref, 4e-6 * (1 + x.to(D).abs()) + h * h / 2)
 
 
+ENDS = [-3.3e38, -1e20, -1e18, -2e13, -1e12, -1e6, -60.0, 60.0, 1e6, 1e12, 2e13, 1e20]
+
+
+@pytest.mark.parametrize("name", [None, "relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("N", [24, 23])
+def test_epilogue_backward_of_large_values(name, dtype, N):
+    """Finite pre-activations however large: the slope is 0 or 1 (silu's at -60 is -5e-25), in d_bias too."""
+    import b2x
+    lim = torch.finfo(dtype).max
+    z = torch.tensor(ENDS + ENDS[::-1], device="cuda").clamp(-lim, lim).to(dtype)[:N].repeat(40, 1)
+    g = randn(40, N, seed=1, dtype=dtype)
+    d, db = b2x.epilogue_backward(g, z, name)
+    ref = g.to(D) * (1.0 if name is None else (z > 0).to(D))
+    check(d, ref, rounded(dtype, ref) + 1e-20, "d_pre")
+    check(db, ref.sum(0), 40 * 2.0 ** -24 * ref.abs().sum(0) + 1e-18, "d_bias")
+
+
+@pytest.mark.parametrize("name", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_gemm_epilogue_of_large_values(name):
+    """The activations themselves there: 0 or the value."""
+    import b2x
+    bias = torch.tensor(ENDS, device="cuda").repeat(11)
+    zero = torch.zeros((5, 128), device="cuda").to(E4)
+    c, pre = b2x.gemm_epilogue(zero, torch.zeros((132, 128), device="cuda").to(E4).t(), bias=bias, activation=name, return_pre=True)
+    check(pre, bias.to(D).expand(5, -1), rounded(BF, bias.to(D)), "pre")
+    ref = bias.to(D).clamp_min(0).expand(5, -1)
+    check(c, ref, rounded(BF, ref) + 1e-20, "C")
+
+
 def test_epilogue_backward_strided_and_in_place_buffers():
     import b2x
     g, z = randn(70, 300, seed=1, dtype=BF)[:, 3:200], randn(197, 70, seed=2, dtype=BF).t()

@@ -129,10 +129,14 @@ __device__ __forceinline__ Pair act_slope(Pair x) {
     const Pair e = exp2_pair(mul2(mul2(x, pair(-0.5f * kLog2E)), x));
     return fma2(mul2(x, pair(0.5f * kGeluA)), e, normal_cdf(x));
   }
-  if constexpr (ACT == B2X_ACT_GELU_TANH) {  // s (1 + x (1 - s) 2 u')
-    const Pair x2 = mul2(x, x), s = sigma2(gelu_tanh_arg(x, x2));
+  if constexpr (ACT == B2X_ACT_GELU_TANH) {
+    // s + x s (1 - s) 2 u': where s is 0 or 1 the product s (1 - s) has to come first, since x (1 - s) 2 u' overflows from
+    // |x| of 1e13 on, and x^2 is held below 1e30 to keep 2 u' finite.  NaN and infinities go through the factor x.
+    float a, b;
+    unpair(mul2(x, x), a, b);
+    const Pair x2 = pair(fminf(a, 1e30f), fminf(b, 1e30f)), s = sigma2(gelu_tanh_arg(x, x2));
     const Pair du = fma2(pair(6.0f * kGeluA * kGeluB), x2, pair(2.0f * kGeluA));
-    return mul2(s, fma2(mul2(x, fma2(s, pair(-1.0f), pair(1.0f))), du, pair(1.0f)));
+    return fma2(mul2(x, mul2(s, fma2(s, pair(-1.0f), pair(1.0f)))), du, s);
   }
   if constexpr (ACT == B2X_ACT_SILU) {  // s (1 + x (1 - s))
     const Pair s = sigma2(mul2(x, pair(-kLog2E)));
