@@ -403,7 +403,9 @@ B2X_API b2x_status b2x_epilogue_backward(const void* grad, int64_t ld_grad, cons
  * lower index.  An expert whose logit or bias is -inf is masked: it is never
  * chosen and weighs nothing; where fewer than top_k experts are left, the
  * remaining slots hold expert -1 and weight 0.  NaN ranks above all numbers
- * and its weight is NaN.  experts <= 1024, top_k <= 32.
+ * and its weight is NaN.  A row whose chosen s are all 0 in 64 bits (sigmoid of
+ * logits below -709, such as the type's lowest value) has weights 0 also where
+ * they are renormalized.  experts <= 1024, top_k <= 32.
  */
 typedef struct {
   const void* logits;

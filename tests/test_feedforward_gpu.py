@@ -419,6 +419,41 @@ def test_route_strided_logits_and_no_tokens():
     assert w.shape == e.shape == (0, 4)
 
 
+@pytest.mark.parametrize("base", [-20.0, -60.0, -88.0, -100.0, -200.0, -600.0])
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_route_sigmoid_of_low_logits(base, dtype):
+    """Renormalised weights sum to the scale however small the scores, and so do their gradients' parts."""
+    import b2x
+    l = (randn(33, 64, seed=3, std=1.5) + base).to(dtype)
+    l[1, 2:] = float("-inf")                     # fewer than k are left
+    l[2, 5] = base / 2                           # one far above the others
+    l[3, 7] = 1.0                                # and one that is not small
+    w, e = check_route(l, 6, "sigmoid", scale=1.7)
+    assert (w.sum(1) - 1.7).abs().max() < 1e-5
+    check_route(l, 6, "sigmoid", groups=8, top_groups=3)
+    g = randn(33, 6, seed=4)
+    got = b2x.moe_route_backward(g, l, e, score="sigmoid", scale=1.7)
+    z = l.to(D).requires_grad_()
+    c = torch.where(e >= 0, torch.sigmoid(z).gather(1, e.clamp_min(0).long()), torch.zeros((), dtype=D, device="cuda"))
+    (1.7 * c / c.sum(1, keepdim=True) * g.to(D)).sum().backward()
+    ref = torch.nan_to_num(z.grad, nan=0.0)
+    check(got, ref, 1e-5 * 1.7 * g.to(D).abs().sum(1, keepdim=True) + rounded(dtype, ref))
+    assert got[4:].abs().amax(1).min() > 1e-7  # nothing vanished
+
+
+def test_route_sigmoid_of_the_lowest_value():
+    """Scores that are 0 in 64 bits too: weights and gradients 0, no NaN; a NaN among them stays one."""
+    import b2x
+    l = torch.full((3, 16), torch.finfo(F32).min, device="cuda")
+    l[1, 4] = float("nan")
+    w, e = check_route(l, 4, "sigmoid")
+    assert (w[0] == 0).all() and torch.isnan(w[1]).all()
+    w, e = check_route(l, 1, "sigmoid")
+    assert torch.isnan(w[1]).all()
+    d = b2x.moe_route_backward(torch.ones((3, 1), device="cuda"), l, e, score="sigmoid")
+    assert (d[0] == 0).all() and (d[2] == 0).all()
+
+
 @pytest.mark.parametrize("T,E,k,score,renorm,dtype", [
     (1, 8, 2, "softmax", True, F32), (33, 64, 8, "softmax", False, F32), (17, 160, 6, "sigmoid", True, BF),
     (9, 1000, 32, "sigmoid", False, F32), (40, 60, 1, "softmax", True, HF), (65, 128, 8, "softmax", False, BF),

@@ -80,6 +80,18 @@ __device__ __forceinline__ float warp_max(float v) {  // of numbers; NaN is igno
   return v;
 }
 
+// sigma(l) of the chosen experts (l = -inf: none), for its quotient by their sum.  sigma(l) is e^l sigma(-l): where all are
+// negative the common factor e^max is left out, so that logits of -90 or -600 give the weights that they give in 64 bits
+// instead of quotients of zeros.  Below kSigmaGone even 1 / (1 + e^-l) in 64 bits is 0 (logits of the type's lowest value): 0.
+constexpr float kSigmaGone = -709.78f;
+__device__ __forceinline__ float sigma_parts(float l) {
+  const bool there = l != -INFINITY;
+  if (__any_sync(kAll, l >= 0.0f)) return there ? sigma_fast(l) : 0.0f;
+  const float top = warp_max(l);  // -inf where all are NaN
+  if (!there) return 0.0f;
+  return top < kSigmaGone ? 0.0f * l : exp_approx(l - top) * sigma_fast(-l);
+}
+
 // The largest (value, lowest index) pair of the warp, in fp64; index INT_MAX: none.
 __device__ __forceinline__ void warp_argmax(double& v, int& at) {
 #pragma unroll
@@ -557,10 +569,12 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
   float w = 0.0f;
   const float lm = mine >= 0 ? load_f32(p.logits, row + mine, p.type) : -INFINITY;
   if (p.sigmoid) {
-    if (mine >= 0) w = sigma_fast(lm);
     if (p.renorm) {
+      w = sigma_parts(lm);
       const float total = warp_sum(w);
       w = total == 0.0f ? 0.0f : __fdiv_rn(w, total);
+    } else if (mine >= 0) {
+      w = sigma_fast(lm);
     }
   } else if (p.renorm) {  // softmax over the chosen ones: the common factor cancels
     const float top = warp_max(lm);
@@ -611,7 +625,7 @@ __device__ __forceinline__ void store_logits(const RouteParams& p, int64_t row, 
 
 // d_logits of one token per warp.  With w_j = scale s_j (/ S, S = sum of the chosen s):
 //   ds_j = scale d_j                              or  scale (d_j - sum_i d_i s_i / S) / S
-//   sigmoid:  dl_e = ds_e s_e (1 - s_e)
+//   sigmoid:  dl_e = ds_e s_e (1 - s_e); renormalised, with p_e = s_e / S,  scale p_e (d_e - sum_i p_i d_i) (1 - s_e)
 //   softmax:  dl_e = s_e (ds_e - sum_i s_i ds_i); renormalised, w / scale is the softmax p over the chosen ones and
 //             dl_e = scale p_e (d_e - sum_i p_i d_i), which needs the chosen logits alone.
 // An expert named in two slots gets the sum of both.  The rest of the row is the dense part (0 except for the
@@ -665,14 +679,15 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_backward_kernel(co
     store_logits<VPL>(p, t * p.ld_d, lane, zero);
     float dl = 0.0f;  // this slot's part
     if (p.sigmoid) {
-      const float s = at >= 0 ? sigma_fast(lm) : 0.0f;
-      const float slope = at >= 0 ? s * sigma_fast(-lm) : 0.0f;
+      const float slope = at >= 0 ? sigma_fast(-lm) : 0.0f;  // of log s
       if (p.renorm) {
-        const float total = warp_sum(s);
-        const float mean = total == 0.0f ? 0.0f : __fdiv_rn(warp_sum(d * s), total);
-        dl = total == 0.0f ? 0.0f : __fdiv_rn((d - mean) * slope, total);
-      } else {
-        dl = d * slope;
+        const float v = sigma_parts(lm);
+        const float total = warp_sum(v);
+        const float pr = total == 0.0f ? 0.0f : __fdiv_rn(v, total);
+        const float mean = warp_sum(at >= 0 ? pr * d : 0.0f);
+        dl = at >= 0 ? pr * (d - mean) * slope : 0.0f;
+      } else if (at >= 0) {
+        dl = d * sigma_fast(lm) * slope;
       }
     } else {
       const float top = warp_max(lm);
