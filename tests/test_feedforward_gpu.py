@@ -410,6 +410,44 @@ def test_route_choices_that_fp32_cannot_tell_apart(E, groups):
     check_route(l, 8, "sigmoid", b, groups, max(1, groups // 2), "top2" if groups > 1 else "max")
 
 
+@pytest.mark.parametrize("E,k", [(64, 6), (64, 32), (256, 8), (24, 3), (1024, 1)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_ties_that_only_64_bits_tell_apart(E, k, score):
+    """Scores that are one number in fp32: at the border of the choice stand experts that are the same, and behind them
+    others, some of them better in 64 bits."""
+    zero = torch.zeros(E, device="cuda")
+    l = torch.zeros((40, E), device="cuda")
+    l[:20] = -600.0 if score == "sigmoid" else -200.0   # all of them 0 in fp32, but for an expert that is not
+    l[:20, 1] = 1.0
+    l[20:] = 1e-4                                       # 1 ulp of the score apart, or less
+    step = torch.where(torch.arange(40, device="cuda") < 20, 4.0, 2e-8)
+    for t in range(40):
+        n = 1 + t % 10
+        at = torch.randperm(E, device="cuda", generator=gen(t))[:n]
+        if t < 20:
+            at = at[at != 1]
+        l[t, at] += step[t]                             # a few above the rest
+        l[t, at[::3]] += step[t]
+    check_route(l, k, score, zero)
+    check_route(l, k, score, zero + 0.25)
+    if E >= 64:
+        check_route(l, k, score, zero, groups=4, top_groups=2, gscore="top2")
+        check_route(l.to(BF), k, score, zero)
+
+
+def test_route_ties_at_the_border_are_not_always_alike():
+    """The last chosen expert and the next one are the same, a third lies within fp32's error of them and is better."""
+    l = torch.full((60, 96), -4.0, device="cuda")
+    for t in range(60):
+        at = torch.randperm(96, device="cuda", generator=gen(t))[:8]
+        l[t, at[:4]] = torch.tensor([3.0, 2.5, 2.0, 1.5], device="cuda")
+        l[t, at[4:7]] = 1.0
+        l[t, at[7]] = 1.0 + (1 + t % 3) * 2.0 ** -23
+    for k in (4, 5, 6, 7, 8):
+        check_route(l, k, "sigmoid", torch.full((96,), 4.0, device="cuda"))
+        check_route(l, k, "softmax", torch.full((96,), 4.0, device="cuda"))
+
+
 def test_route_strided_logits_and_no_tokens():
     import b2x
     l = randn(30, 200, seed=1)

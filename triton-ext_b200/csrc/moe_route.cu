@@ -531,26 +531,36 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
         if (e0 + i == e) key[i] = 0;
       if (lane == j) my_key = best, at = e;
     }
-    if (p.k == 32 && p.bias) {  // no lane is left to hold the 33rd: compare it here
-      int e;
-      const uint32_t best = take_max<VPL>(key, lane, e);
-      const uint32_t last = __shfl_sync(kAll, my_key, 31);
-      if (best != 0 && last < kNaN && near(last, best, 1.0f)) close = true;
-    }
   }
   bool swap = false;  // neighbours to be told apart in fp64, all among the candidates
   if (p.bias) {
-    // neighbours in the order that fp32 cannot tell apart, unless logits and biases are the same: then the index decides
+    // Neighbours in the order that fp32 cannot tell apart, unless logits and biases are the same: then the index decides.
+    // The k-th may stand at the head of a run of such neighbours (some of them the same), and any of them may belong
+    // before it: the whole run counts, and where it may go on outside the candidates what is left is compared too.
     const uint32_t next_key = __shfl_down_sync(kAll, my_key, 1);
     const int next_at = __shfl_down_sync(kAll, at, 1);
-    if (lane < p.k && lane < 31 && my_key != 0 && next_key != 0 && my_key != kNaN && next_key != kNaN &&
-        near(my_key, next_key, 1.0f)) {
+    const bool run = lane < 31 && my_key != 0 && next_key != 0 && my_key != kNaN && next_key != kNaN && near(my_key, next_key, 1.0f);
+    bool differ = false;
+    if (run) {
       const float la = load_f32(p.logits, row + at, p.type), lb = load_f32(p.logits, row + next_at, p.type);
-      if (!(la == lb && __ldg(p.bias + at) == __ldg(p.bias + next_at))) swap = true;
+      differ = !(la == lb && __ldg(p.bias + at) == __ldg(p.bias + next_at));
+    }
+    const uint32_t runs = __ballot_sync(kAll, run), differs = __ballot_sync(kAll, differ);
+    const int end = p.k - 2 + __ffs(~(runs >> (p.k - 1)));  // last lane of the k-th's run
+    swap = (differs & ((1u << end) - 1)) != 0;
+    const uint32_t last = __shfl_sync(kAll, my_key, p.k - 1);
+    if (last != 0 && last < kNaN &&
+        (n > 32 ? p.k == 32 || end >= p.k : end >= p.k && bound > 1 && near(max(last, bound), bound, 1.0f))) {
+      const int last_at = __shfl_sync(kAll, at, p.k - 1);
+      const float ll = load_f32(p.logits, row + last_at, p.type), lb = __ldg(p.bias + last_at);
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (key[i] != 0 && (n > 32 || key[i] < bound) && near(last, key[i], 1.0f))
+          close = close || !(load_f32(p.logits, row + e0 + i, p.type) == ll && __ldg(p.bias + e0 + i) == lb);
     }
   }
   close = __any_sync(kAll, close);
-  if (__any_sync(kAll, swap) && !close) {
+  if (swap && !close) {
     const uint32_t last = __shfl_sync(kAll, my_key, p.k - 1);
     if (n > 32 || (last != 0 && last < kNaN && near(max(last, bound), bound, 1.0f))) {
       close = true;  // values below the bound may belong to the choice
