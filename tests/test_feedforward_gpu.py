@@ -448,6 +448,57 @@ def test_route_ties_at_the_border_are_not_always_alike():
         check_route(l, k, "softmax", torch.full((96,), 4.0, device="cuda"))
 
 
+def route_choice_64(l, bias, k, score, groups, top_groups):
+    """Experts by top-2 group scores, in 64 bits on the GPU (many rows)."""
+    s = torch.sigmoid(l.to(D)) if score == "sigmoid" else torch.softmax(l.to(D), 1)
+    c = s + bias.to(D)
+    T, E = l.shape
+    two = torch.sort(c.view(T, groups, -1), dim=2, descending=True)[0][:, :, :2].sum(2)
+    best = torch.sort(two, dim=1, descending=True, stable=True)[1][:, :top_groups]
+    kept = torch.zeros_like(two, dtype=torch.bool).scatter_(1, best, True).repeat_interleave(E // groups, 1)
+    return torch.sort(c.masked_fill(~kept, float("-inf")), dim=1, descending=True, stable=True)[1][:, :k].to(torch.int32)
+
+
+@pytest.mark.parametrize("E,groups", [(256, 128), (256, 32), (1024, 16), (96, 16), (24, 12)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_groups_whose_two_choices_cancel(E, groups, score):
+    """Biases +b and -b in every group: the sum of the two is small beside the roundings of its terms."""
+    import b2x
+    gs = E // groups
+    for b in (0.5, 4.0, 16.0, 100.0, 1e4):
+        bias = torch.full((groups, gs), -3.0 * b, device="cuda")
+        bias[:, 0], bias[:, 1] = b, -b
+        l = randn(8000, E, seed=int(b), std=1.5)
+        k = min(8, groups // 2)
+        _, e = b2x.moe_route(l, k, score=score, bias=bias.view(-1), num_groups=groups, top_groups=k, group_score="top2")
+        ref = route_choice_64(l, bias.view(-1), k, score, groups, k)
+        assert int((e != ref).any(1).sum()) == 0, b
+
+
+def test_route_groups_with_one_far_larger_bias():
+    """The uncertain group need not be the next one: one of large terms may stand far behind it in fp32."""
+    import b2x
+    E, groups = 64, 8
+    l = randn(8000, E, seed=5, std=1e-2)
+    bias = torch.zeros((groups, 8), device="cuda")
+    bias[::2, 0], bias[::2, 1], bias[::2, 2:] = 3e4, -3e4, -1e5   # half of the groups: s1 + s2 after cancellation
+    _, e = b2x.moe_route(l, 4, score="softmax", bias=bias.view(-1), num_groups=groups, top_groups=4, group_score="top2")
+    assert torch.equal(e, route_choice_64(l, bias.view(-1), 4, "softmax", groups, 4))
+
+
+@pytest.mark.parametrize("E,groups", [(32, 8), (256, 8), (96, 16), (60, 5)])
+def test_route_groups_of_the_lowest_bias(E, groups):
+    """Experts that a bias of the type's lowest value puts last are still experts: their groups are not empty."""
+    l = randn(9, E, seed=1)
+    bias = torch.zeros((groups, E // groups), device="cuda")
+    bias[2:] = torch.finfo(F32).min
+    k = min(32, 3 * (E // groups) - 1)
+    for score in ("softmax", "sigmoid"):
+        _, e = check_route(l, k, score, bias.view(-1), groups, 4, "top2")
+        check_route(l, k, score, bias.view(-1), groups, 4, "max")
+        assert (e >= 0).all()
+
+
 def test_route_strided_logits_and_no_tokens():
     import b2x
     l = randn(30, 200, seed=1)

@@ -13,8 +13,8 @@
 // exact.  With a bias (and for sums of two) the keys are fp32 values of s + b.  s is off by at most err = 2^-20 (sigmoid) or
 // (2^-20 + (VPL + 5) 2^-24) max s: the approximate exponential and reciprocal together stay below 2^-20 relative and the
 // softmax's sum adds VPL + 5 roundings; s + b is rounded once, by 2^-24 of it.  A row in which two neighbours of the
-// order a, b lie closer than 2 err + 2^-23 (|a| + |b|), or the group scores at the border closer than twice that, is
-// settled in fp64: the groups alone (groups_exact), the candidates' order alone (rank_exact), or, where neither will do,
+// order a, b lie closer than 2 err + 2^-23 (|a| + |b|), or in which a group that goes may be off by as much as sets it
+// behind one that stays (2 err and 2^-24 of its two choices and of their sum, each), is settled in fp64: the groups alone (groups_exact), the candidates' order alone (rank_exact), or, where neither will do,
 // the whole choice (choose_exact).  It is right to fp64, at the speed of fp32 for nearly all rows (16384 tokens, 256
 // experts, k = 8: 34 rows needed it; settling them all by choose_exact took the kernel from 24 to 31 us).
 //
@@ -22,6 +22,7 @@
 // their two largest 17 / 20 / 24 / 30 us.  8 tokens: 2.7 to 4.0 us, launch and latency.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cfloat>
 #include <cstdint>
 #include "activations.cuh"
 #include "b2x_internal.h"
@@ -390,10 +391,25 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
 #pragma unroll
     for (int i = 0; i < VPL; ++i) gkey[i] = key[i] = order_key(l[i]);
   }
-  auto near = [&](uint32_t a, uint32_t b, float scale) {  // a >= b, both numbers
+  auto near = [&](uint32_t a, uint32_t b) {  // a >= b, both numbers
     const float x = key_value(a), y = key_value(b);
-    return !(x - y > scale * fmaf(0x1p-23f, fabsf(x) + fabsf(y), 2.0f * err));
+    return !(x - y > fmaf(0x1p-23f, fabsf(x) + fabsf(y), 2.0f * err));
   };
+  // A group's score from the keys of its two best choices, and how far it may be off: each s by err, each s + b and the sum
+  // of the two by 2^-24 of itself, however little of them the sum leaves (doubled, for the roundings of the limits below).
+  auto group_score = [&](uint32_t a, uint32_t b, float& slack) -> uint32_t {
+    if (!values || a == 0) return a;
+    if (a == kNaN) return kNaN;  // b is not above a
+    const float x = key_value(a), y = p.top2 && b != 0 ? key_value(b) : 0.0f;
+    slack = fmaf(0x1p-22f, fabsf(x) + fabsf(y), 2.0f * err);
+    return p.top2 && b != 0 ? order_key(fmaxf(x + y, -FLT_MAX)) : a;  // two of the lowest value are no masked group
+  };
+  constexpr uint32_t kTop = 0xffffffffu;
+  auto lowest = [&](uint32_t score, float slack) { return score == kNaN ? kTop : order_key(fmaxf(key_value(score) - slack, -FLT_MAX)); };
+  auto highest = [&](uint32_t score, float slack) { return score == kNaN ? kTop : order_key(key_value(score) + slack); };
+  // Whether a group that goes may belong before one that stays: `last` is the least of what those may be that stay, `next`
+  // the most of the others (0: there is none; kTop: NaN alone, told apart by their index).
+  auto border = [&](uint32_t last, uint32_t next) { return next != 0 && next != kTop && last != kTop && last <= next; };
   bool close = false;  // something to be told apart in fp64
   if (p.groups > 1) {
     const int gs = p.E / p.groups;
@@ -407,8 +423,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
         if (p.top2) b = max(min(a, a2), max(b, __shfl_xor_sync(kAll, b, o)));
         a = max(a, a2);
       }
-      uint32_t score = a;
-      if (p.top2 && b != 0) score = a == kNaN || b == kNaN ? kNaN : order_key(key_value(a) + key_value(b));
+      float slack = 0.0f;
+      const uint32_t score = group_score(a, b, slack);
       const int g = lane / p.lanes_per_group;
       int better = 0;
       for (int i = 0; i < p.groups; ++i) {
@@ -416,18 +432,19 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
         better += other > score || (other == score && i < g);
       }
       bool kept = score != 0 && g < p.groups && better < p.top_groups;
-      if (values) {  // the border between the groups that stay and those that go
-        const uint32_t last = __reduce_min_sync(kAll, kept ? score : 0xffffffffu);
-        const uint32_t next = __reduce_max_sync(kAll, !kept && g < p.groups ? score : 0u);
-        if (next != 0 && last < kNaN && next < kNaN && near(last, next, 2.0f)) kept = groups_exact<VPL>(p, row, lane);
+      if (values) {
+        const uint32_t last = __reduce_min_sync(kAll, kept ? lowest(score, slack) : kTop);
+        const uint32_t next = __reduce_max_sync(kAll, !kept && score != 0 && g < p.groups ? highest(score, slack) : 0u);
+        if (border(last, next)) kept = groups_exact<VPL>(p, row, lane);
       }
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
         if (!kept) key[i] = 0;
     } else {
       uint32_t gk[VPL];  // lane l: groups VPL l ..
+      float gs_off[VPL];
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) gk[i] = 0;
+      for (int i = 0; i < VPL; ++i) gk[i] = 0, gs_off[i] = 0.0f;
       for (int g = 0; g < p.groups; ++g) {
         uint32_t a = 0, b = 0;  // the lane's two largest of the group
         const int lo = g * gs - e0, hi = lo + gs;
@@ -437,36 +454,38 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
           b = max(b, min(a, v));
           a = max(a, v);
         }
-        uint32_t score = __reduce_max_sync(kAll, a);
+        const uint32_t best = __reduce_max_sync(kAll, a);
+        uint32_t second = 0;
         if (p.top2) {
-          const uint32_t who = __ballot_sync(kAll, a == score);
-          const uint32_t second = __reduce_max_sync(kAll, lane == __ffs(who) - 1 ? b : a);
-          if (second != 0) score = score == kNaN || second == kNaN ? kNaN : order_key(key_value(score) + key_value(second));
+          const uint32_t who = __ballot_sync(kAll, a == best);
+          second = __reduce_max_sync(kAll, lane == __ffs(who) - 1 ? b : a);
         }
+        float slack = 0.0f;
+        const uint32_t score = group_score(best, second, slack);
 #pragma unroll
         for (int i = 0; i < VPL; ++i)
-          if (e0 + i == g) gk[i] = score;
+          if (e0 + i == g) gk[i] = score, gs_off[i] = slack;
       }
       bool kept[VPL];
 #pragma unroll
       for (int i = 0; i < VPL; ++i) kept[i] = false;
-      uint32_t last = 0;
+      uint32_t last = kTop;
       for (int n = 0; n < p.top_groups; ++n) {
         int at;
-        const uint32_t best = take_max<VPL>(gk, lane, at);
-        if (best == 0) break;
-        last = best;
+        if (take_max<VPL>(gk, lane, at) == 0) break;
         const int lo = at * gs - e0, hi = lo + gs;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-          if (e0 + i == at) gk[i] = 0;
+          if (e0 + i == at) last = min(last, lowest(gk[i], gs_off[i])), gk[i] = 0;
           if (i >= lo && i < hi) kept[i] = true;
         }
       }
-      if (values && last != 0) {
-        int at;
-        const uint32_t next = take_max<VPL>(gk, lane, at);
-        if (next != 0 && last < kNaN && next < kNaN) close = near(last, next, 2.0f);
+      if (values) {
+        uint32_t next = 0;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+          if (gk[i] != 0) next = max(next, highest(gk[i], gs_off[i]));
+        close = border(__reduce_min_sync(kAll, last), __reduce_max_sync(kAll, next));
       }
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
@@ -539,7 +558,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
     // before it: the whole run counts, and where it may go on outside the candidates what is left is compared too.
     const uint32_t next_key = __shfl_down_sync(kAll, my_key, 1);
     const int next_at = __shfl_down_sync(kAll, at, 1);
-    const bool run = lane < 31 && my_key != 0 && next_key != 0 && my_key != kNaN && next_key != kNaN && near(my_key, next_key, 1.0f);
+    const bool run = lane < 31 && my_key != 0 && next_key != 0 && my_key != kNaN && next_key != kNaN && near(my_key, next_key);
     bool differ = false;
     if (run) {
       const float la = load_f32(p.logits, row + at, p.type), lb = load_f32(p.logits, row + next_at, p.type);
@@ -550,19 +569,19 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 12 : (VPL <= 16 ?
     swap = (differs & ((1u << end) - 1)) != 0;
     const uint32_t last = __shfl_sync(kAll, my_key, p.k - 1);
     if (last != 0 && last < kNaN &&
-        (n > 32 ? p.k == 32 || end >= p.k : end >= p.k && bound > 1 && near(max(last, bound), bound, 1.0f))) {
+        (n > 32 ? p.k == 32 || end >= p.k : end >= p.k && bound > 1 && near(max(last, bound), bound))) {
       const int last_at = __shfl_sync(kAll, at, p.k - 1);
       const float ll = load_f32(p.logits, row + last_at, p.type), lb = __ldg(p.bias + last_at);
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
-        if (key[i] != 0 && (n > 32 || key[i] < bound) && near(last, key[i], 1.0f))
+        if (key[i] != 0 && (n > 32 || key[i] < bound) && near(last, key[i]))
           close = close || !(load_f32(p.logits, row + e0 + i, p.type) == ll && __ldg(p.bias + e0 + i) == lb);
     }
   }
   close = __any_sync(kAll, close);
   if (swap && !close) {
     const uint32_t last = __shfl_sync(kAll, my_key, p.k - 1);
-    if (n > 32 || (last != 0 && last < kNaN && near(max(last, bound), bound, 1.0f))) {
+    if (n > 32 || (last != 0 && last < kNaN && near(max(last, bound), bound))) {
       close = true;  // values below the bound may belong to the choice
     } else {
       const int better = rank_exact<VPL>(p, row, lane, at, lane < n);
