@@ -499,6 +499,29 @@ def test_route_groups_of_the_lowest_bias(E, groups):
         assert (e >= 0).all()
 
 
+@pytest.mark.parametrize("E,k", [(24, 4), (64, 8), (256, 8), (1024, 32)])
+@pytest.mark.parametrize("std,base", [(1.5, 0.0), (15.0, 0.0), (3.0, -20.0), (1.5, -80.0), (30.0, 7.3)])
+def test_route_weights_to_a_few_units(E, k, std, base):
+    """u = 2^-24.  The exponential is off by 2 units in the last place (4 u), with the difference put back 5 u; 1 + e by
+    3 u; each division, product and level of the warp's sum by u.
+      sigmoid              8 u, scale u                                               9 u
+      sigmoid, quotient    9 u above; 9 u and 5 levels below; division, scale         25 u
+      softmax of the k     5 u above; 5 u and 5 levels below; division, scale         17 u
+      softmax of all       5 u above; below each term by 4 u (2^-22, the approximate exponential) and by 3 u of its distance
+                           from the maximum, which in the mean over the softmax is at most ln E; levels 5 and experts a
+                           lane at most 2 ceil(E / 32); division, scale               (16 + 5 + 3 ln E + 2 ceil(E / 32)) u"""
+    import b2x
+    u = 2.0 ** -24
+    l = randn(200, E, seed=E, std=std) + base
+    for score, renorm, bound in (("sigmoid", False, 9), ("sigmoid", True, 25), ("softmax", True, 17),
+                                 ("softmax", False, 21 + 3 * np.log(E) + 2 * -(-E // 32))):
+        w, e = b2x.moe_route(l, k, score=score, renormalize=renorm, scale=1.7)
+        s = torch.sigmoid(l.to(D)) if score == "sigmoid" else torch.softmax(l.to(D), 1)
+        c = s.gather(1, e.long())
+        ref = float(np.float32(1.7)) * (c / c.sum(1, keepdim=True) if renorm else c)
+        check(w, ref, bound * u * ref + 2.0 ** -146, (score, renorm))
+
+
 def test_route_strided_logits_and_no_tokens():
     import b2x
     l = randn(30, 200, seed=1)
