@@ -225,6 +225,26 @@ def test_epilogue_backward_against_differences(name):
     check(d, ref, 4e-6 * (1 + x.to(D).abs()) + h * h / 2)
 
 
+@pytest.mark.parametrize("name,bound", [("gelu", 12), ("gelu_tanh", 16), ("silu", 10), ("relu", 0), (None, 0)])
+@pytest.mark.parametrize("N", [512, 257])
+def test_epilogue_backward_fp32_to_a_few_units(name, bound, N):
+    """u = 2^-24; the exponential is off by 4 u (2 units in the last place, or 2^-22 for the approximate one).
+      gelu       erfc(|x|) / 2 <= 0.5: its fit 2 u, the exponential 4 u, the polynomial's rounding 8 u, z^2 1 u; x phi(x) <=
+                 0.25 by 8 u; the differences and sums 2 u
+      silu       e^-|x| 4 u, 1 / (1 + e) 4 u, their product 9 u; x q <= 0.28 and the sum by 10 u and u, the product by s
+      gelu_tanh  the exponent y by 5 u y, y e^-y <= 0.37: sigma 5 u; x p q 2u' <= 0.35 by 21 u + 5 u y; the sum 1.1 u"""
+    import b2x
+    u = 2.0 ** -24
+    z = torch.linspace(-20, 20, 300 * N, device="cuda").view(300, N)
+    z = torch.cat([z, z * 2.0 ** -8])
+    g = randn(600, N, seed=1)
+    d, db = b2x.epilogue_backward(g, z, name)
+    ref = g.to(D) * (slope(z.to(D), name) if name else 1.0)
+    tol = bound * u * g.to(D).abs() + u * ref.abs() + 2.0 ** -126
+    check(d, ref, tol, "d_pre")
+    check(db, ref.sum(0), tol.sum(0) + 600 * u * ref.abs().sum(0), "d_bias")
+
+
 ENDS = [-3.3e38, -1e20, -1e18, -2e13, -1e12, -1e6, -60.0, 60.0, 1e6, 1e12, 2e13, 1e20]
 
 

@@ -6,7 +6,8 @@
 // is no workspace and no atomic.  The rows come through a ring in shared memory that each thread fills for itself ahead
 // (cp.async): loads into registers left too few bytes on the way beside the slope's own registers.
 // Bound: HBM, three times the matrix, and the instructions of the slope: 4000 x 28672 bf16 gelu_tanh 120 us (5.7 TB/s; with
-// loads into registers 126, with single fp32 operations besides 248), gelu 147 us; 8192 x 1024 silu 12 us.
+// loads into registers 126, with single fp32 operations besides 248), gelu 147 us; 8192 x 1024 silu 12 us;
+// 4000 x 28672 fp32, twice the bytes: gelu_tanh 226 us, gelu 221.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
@@ -30,6 +31,18 @@ struct EpiBwdParams {
   float* d_bias;
   int64_t rows, cols;
 };
+
+// The slope of values of type T, two at a time.
+template <typename T, int ACT>
+__device__ __forceinline__ Pair slope_of(Pair x) {
+  if constexpr (sizeof(T) == 4 && (ACT == B2X_ACT_GELU_TANH || ACT == B2X_ACT_SILU)) {
+    float a, b;
+    unpair(x, a, b);
+    return pair(act_slope_f32<ACT>(a), act_slope_f32<ACT>(b));
+  } else {
+    return act_slope<ACT>(x);
+  }
+}
 
 // 16 bytes from global to shared memory, past L1 (d_pre may be grad or pre: a thread reads its values before it writes
 // them, and no other thread touches them).
@@ -70,7 +83,7 @@ __global__ void __launch_bounds__(kEbThreads, 4) epilogue_backward_kernel(const 
           const int64_t ru = r + (int64_t)u * TY;
           if (ru < r1) {
             float d, none;
-            unpair(act_slope<ACT>(pair(to_f32(zv[u]))), d, none);
+            unpair(slope_of<T, ACT>(pair(to_f32(zv[u]))), d, none);
             d *= to_f32(gv[u]);
             sum[0] += d;
             o[ru * p.ld_out] = from_f32<T>(d);
@@ -111,7 +124,7 @@ __global__ void __launch_bounds__(kEbThreads, 4) epilogue_backward_kernel(const 
 #pragma unroll
           for (int i = 0; i < V; i += 2) {
             const Pair z2 = pair(to_f32(zv.e[i]), to_f32(zv.e[i + 1]));
-            const Pair d2 = mul2(pair(to_f32(gv.e[i]), to_f32(gv.e[i + 1])), act_slope<ACT>(z2));
+            const Pair d2 = mul2(pair(to_f32(gv.e[i]), to_f32(gv.e[i + 1])), slope_of<T, ACT>(z2));
             float a, b;
             unpair(add2(pair(sum[i], sum[i + 1]), d2), sum[i], sum[i + 1]);
             unpair(d2, a, b);
