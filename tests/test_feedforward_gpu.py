@@ -275,6 +275,49 @@ def test_gemm_epilogue_of_large_values(name):
     check(c, ref, rounded(BF, ref) + 1e-20, "C")
 
 
+# wide enough for 8 and for 32 threads side by side (296 and 1184 runs of 16 bytes on 148 SMs), the last block partly empty,
+# several rounds of the ring, rows split over a cluster or not
+@pytest.mark.parametrize("M,N,name,dtype", [(4100, 2400, "gelu", BF), (300, 2400, "silu", HF), (301, 9480, "gelu_tanh", BF), (1, 9480, "relu", HF),
+                                            (1300, 9480, None, BF), (70, 4800, "silu", F32), (900, 1200, "gelu_tanh", F32),
+                                            (3, 19000, "gelu", BF)])
+def test_epilogue_backward_wide(M, N, name, dtype):
+    test_epilogue_backward(M, N, name, dtype)
+
+
+@pytest.mark.parametrize("M,N", [(1100, 2400), (600, 9480), (257, 264), (130, 33)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_epilogue_backward_in_place(M, N, dtype):
+    """d_pre may be grad or pre: the bits of the call with an output of its own."""
+    import b2x
+    from b2x import _lib as L
+    g, z = randn(M, N, seed=1, dtype=dtype), randn(M, N, seed=2, dtype=dtype)
+    kind = {BF: L.BF16, F32: L.F32}[dtype]
+    for act_id, name in ((0, None), (2, "gelu"), (3, "gelu_tanh")):
+        want, db = b2x.epilogue_backward(g, z, name)
+        for over in ("grad", "pre"):
+            a, b = g.clone(), z.clone()
+            out = a if over == "grad" else b
+            got = torch.empty_like(db)
+            L.check(L.lib().b2x_epilogue_backward(a.data_ptr(), N, b.data_ptr(), N, out.data_ptr(), N, got.data_ptr(), kind, M, N, act_id,
+                                                  torch.cuda.current_stream().cuda_stream))
+            assert torch.equal(out, want) and torch.equal(got, db), (name, over)
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 256, 4096), (70, 520, 512), (1025, 2304, 512), (700, 1037, 256)])
+@pytest.mark.parametrize("out", [BF, HF])
+def test_gemm_epilogue_onto_its_residual(M, N, K, out):
+    """The residual may be C itself, on either product kernel and with rows off the 8-byte grid."""
+    import b2x
+    from b2x import _lib as L
+    a, b, bias = fp8(M, K, seed=1, std=1.0), fp8(N, K, seed=2, std=0.1), randn(N, seed=3)
+    c = randn(M, N, seed=4, dtype=out)
+    want = b2x.gemm_epilogue(a, b.t(), bias=bias, activation="gelu", residual=c, out_dtype=out)
+    g = L.GemmArgs(a.data_ptr(), b.data_ptr(), c.data_ptr(), M, N, K, K, 1, K, N, L.E4M3, L.E4M3, L.BF16 if out == BF else L.F16)
+    ep = L.Epilogue(bias=bias.data_ptr(), bias_type=L.F32, activation=2, residual=c.data_ptr(), ld_residual=N)
+    L.check(L.lib().b2x_fp8_gemm_epilogue(L.ctypes.byref(g), L.ctypes.byref(ep), torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(c, want)
+
+
 def test_epilogue_backward_strided_and_in_place_buffers():
     import b2x
     g, z = randn(70, 300, seed=1, dtype=BF)[:, 3:200], randn(197, 70, seed=2, dtype=BF).t()
@@ -586,6 +629,17 @@ def test_route_sigmoid_of_the_lowest_value():
     assert (d[0] == 0).all() and (d[2] == 0).all()
 
 
+@pytest.mark.parametrize("E", [192, 320, 352, 512, 768])
+@pytest.mark.parametrize("score,dtype", [("sigmoid", F32), ("softmax", BF)])
+def test_route_of_other_widths(E, score, dtype):
+    """6, 10, 12, 16 and 32 experts a lane, with and without bias and groups, forward and backward."""
+    test_route(20, E, 8, score, True, 16, 5, "top2", True, dtype)
+    test_route(20, E, 8, score, False, 16, 5, "max", False, dtype)
+    test_route(20, E, 31, score, True, 1, 1, "max", False, dtype)
+    test_route_backward(20, E, 8, score, True, dtype)
+    test_route_backward(20, E, 8, score, False, dtype)
+
+
 @pytest.mark.parametrize("T,E,k,score,renorm,dtype", [
     (1, 8, 2, "softmax", True, F32), (33, 64, 8, "softmax", False, F32), (17, 160, 6, "sigmoid", True, BF),
     (9, 1000, 32, "sigmoid", False, F32), (40, 60, 1, "softmax", True, HF), (65, 128, 8, "softmax", False, BF),
@@ -703,6 +757,13 @@ def test_dispatch(T, H, E, k, dtype, q):
     check_dispatch(x, e, E, q)
     e[:] = -1                # nothing left
     check_dispatch(x, e, E, q)
+
+
+@pytest.mark.parametrize("T,k", [(8193, 8), (16385, 8), (140000, 1)])
+def test_dispatch_of_many_pairs(T, k):
+    """More than 65536 pairs: the plan's warps take several rounds."""
+    e = torch.randint(-2, 70, (T, k), device="cuda", generator=gen(5), dtype=torch.int32)
+    check_dispatch(randn(T, 16, seed=T, dtype=BF), e, 64)
 
 
 def test_dispatch_special_values_strides_and_wide_integers():
@@ -913,6 +974,13 @@ def test_combine_and_backward(T, k, H, dtype):
     check(dy, ref, rounded(dtype, ref) + 2.0 ** -24 * ref.abs(), "d_y")
     prod = yr * g.to(D)[:, None, :]
     check(dw, prod.sum(2), H * 2.0 ** -24 * prod.abs().sum(2) + 1e-30, "d_weights")
+
+
+# several column steps and several CTAs a token; more of them than go side by side (the second and the last two)
+@pytest.mark.parametrize("T,k,H,dtype", [(60, 8, 7168, BF), (22000, 2, 2056, BF), (50, 9, 7168, HF), (33, 3, 4500, F32), (3000, 4, 2049, BF),
+                                         (2500, 1, 1030, F32)])
+def test_combine_and_backward_wide(T, k, H, dtype):
+    test_combine_and_backward(T, k, H, dtype)
 
 
 def test_combine_backward_against_differences():
