@@ -275,3 +275,21 @@ def test_values_off_their_own_grid_are_refused():
     ok = [P, 64, P, 64, P, 64, P, 0, 4, 64, 0]
     for at in (0, 2, 4):
         refused("b2x_epilogue_backward", "ERR_INVALID_ARG", *[P + 2 if i == at else a for i, a in enumerate(ok)])
+
+
+def test_counts_past_32_bits_are_refused():
+    """num_groups = 2^32 + 1 would reach the C ABI as 1."""
+    from b2x.feedforward import _count
+    for v in (1 << 31, (1 << 32) + 1, -(1 << 31) - 1):
+        with pytest.raises(ValueError, match="32 bits"):
+            _count(v, "num_groups")
+    assert _count(8, "num_groups") == 8 and _count(-1, "top_k") == -1
+
+
+@pytest.mark.gpu
+def test_route_refuses_counts_past_32_bits():
+    import b2x
+    x = torch.zeros((4, 8), device="cuda")
+    for kw in (dict(top_k=(1 << 32) + 2), dict(top_k=2, num_groups=(1 << 32) + 1), dict(top_k=2, num_groups=2, top_groups=(1 << 32) + 1)):
+        with pytest.raises(ValueError, match="32 bits"):
+            b2x.moe_route(x, **kw)

@@ -240,6 +240,13 @@ def _choice(table: dict, value, what: str) -> int:
     return table[value]
 
 
+def _count(value: int, what: str) -> int:
+    """A number that the C ABI takes as int, which would wrap past 32 bits."""
+    if not -2**31 <= value < 2**31:
+        raise ValueError(f"{what} must fit 32 bits, got {value}")
+    return value
+
+
 def moe_route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Optional[torch.Tensor] = None,
               num_groups: int = 1, top_groups: int = 1, group_score: str = "max", renormalize: bool = True,
               scale: float = 1.0):
@@ -256,11 +263,11 @@ def moe_route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias:
     logits = _rows(logits, "logits")
     T, E = logits.shape
     bias = _scale(bias, "bias", E)
-    k = max(top_k, 0)
+    k = max(_count(top_k, "top_k"), 0)
     weights = logits.new_empty((T, k), dtype=torch.float32)
     experts = logits.new_empty((T, k), dtype=torch.int32)
     a = L.MoeRouteArgs(logits.data_ptr(), FLOAT_DTYPES[logits.dtype], T, E, _ld(logits), top_k, _choice(SCORES, score, "score"),
-                       None if bias is None else bias.data_ptr(), num_groups, top_groups,
+                       None if bias is None else bias.data_ptr(), _count(num_groups, "num_groups"), _count(top_groups, "top_groups"),
                        _choice(GROUP_SCORES, group_score, "group_score"), bool(renormalize), scale, weights.data_ptr(),
                        experts.data_ptr())
     _call(dev, L.lib().b2x_moe_route, _byref(a))
