@@ -11,6 +11,10 @@ A mixture-of-experts layer is route -> dispatch -> moe_gemm_swiglu -> moe_gemm -
 the whole run can be captured into a CUDA graph.  All arithmetic happens in the sm_100a kernels of libb2x.so (C ABI in
 include/b2x.h); there is no CPU path.  The calls run on the current stream of their tensors' device and keep no state
 between them.
+
+Where the rows of a new result are no multiple of 16 bytes, it is a view of rows padded to one (strides as it says, not
+contiguous).  float8 operands whose rows do not start on 16-byte boundaries are copied to padded rows in every call; a
+weight that is kept spares that where it is stored padded: torch.empty(N, -(-K // 16) * 16)[:, :K].
 """
 from __future__ import annotations
 
@@ -256,7 +260,8 @@ def moe_route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias:
     by the chosen ones' sum if renormalize, times scale.  With num_groups > 1 only the experts of the top_groups best
     groups take part; a group scores its largest ("max") or the sum of its two largest ("top2") choices.  The slots fall
     in choice, equal choices go to the lower expert.  An expert with logit or bias -inf is masked; slots that no expert
-    is left for hold expert -1 and weight 0, which moe_dispatch drops.  E <= 1024, top_k <= 32."""
+    is left for hold expert -1 and weight 0, which moe_dispatch drops.  Sigmoid scores that are 0 in 64 bits (logits of the
+    type's lowest value) weigh 0 also where renormalized.  E <= 1024, top_k <= 32."""
     dev = _device(logits, bias)
     if logits.dtype not in FLOAT_DTYPES:
         raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")

@@ -6,7 +6,7 @@
 // behind the other's stream).  The K ranges of a tile are the CTAs of a cluster: each leaves its fp32 partial tile in its
 // own shared memory and the cluster adds them over distributed shared memory in the order of the ranges, so there is no
 // workspace, no atomic, nothing to clear, and the same inputs give the same bits.  For few tokens it is bound by reading
-// the weights once: 1 x 8192 x 28672 in 43 us (5.4 TB/s), 40 rows on 64 experts of 7168 x 2048 in 77 us (5.7 TB/s).
+// the weights once: 1 x 8192 x 28672 in 42 us (5.6 TB/s), 40 rows on 64 experts of 7168 x 2048 in 71 to 75 us (5.9 TB/s).
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -249,7 +249,8 @@ __global__ void __launch_bounds__(kTkThreads, 2)
 // four.  The other roles only read the ring: when each searched for its units itself, with the divisions and shuffles
 // that takes, the loads and MMAs stood still for some 4000 cycles at every change of unit.
 //
-// Bound by the tensor cores under the power cap.  Measured (a few launches after an idle gap): 4000 x 28672 x 8192 in 689 us
+// Bound by the tensor cores under the power cap.  Measured (a few launches after an idle gap; back to back, at the clock that
+// the cap leaves, the second takes 815 to 840 us and the experts' 600 to 620): 4000 x 28672 x 8192 in 689 us
 // (the plain paired GEMM: 672), with bias, gelu_tanh and pre 739; 8192^3 in 402 (385); 20001 rows on 32 experts of
 // 4096 x 7168 with SwiGLU in 511 us, of which the narrower tiles cost most: the time follows the columns, 64 to 256.
 
@@ -747,8 +748,8 @@ static b2x_status launch_tokens(TokLaunch& g, const char* who, cudaStream_t st) 
   const int64_t tok_tiles = moe ? p.rows / nt + std::min<int64_t>(p.E, p.rows) : (p.rows + nt - 1) / nt;
   const int64_t units = tok_tiles * p.n_tiles;
   const double planned = std::max(1.0, moe ? active * ceil(mean / nt) : (double)tok_tiles) * p.n_tiles;
-  // K ranges: none if the tiles reach every SM, else the fewest that do, but 8 only where 4 would leave more than half
-  // of the SMs idle: a larger cluster costs more to place and to add up (1 x 28672 x 8192, 224 tiles: 42 us with one
+  // K ranges: none if the tiles reach every SM, else the fewest that do, but 8 only where 4 give fewer than 64 CTAs (a little
+  // under half of the SMs): a larger cluster costs more to place and to add up (1 x 28672 x 8192, 224 tiles: 42 us with one
   // range, 44, 52 and 60 with 2, 4 and 8; 1 x 8192 x 8192, 64 tiles: 23, 14.5, 11.2, 16; 1 x 1024 x 16384, 8 tiles: 41, 23,
   // 13.8, 9.5).
   p.splits = 1;
@@ -760,9 +761,11 @@ static b2x_status launch_tokens(TokLaunch& g, const char* who, cudaStream_t st) 
   }
   if (units * p.splits >= (1LL << 31)) return fail(B2X_ERR_UNSUPPORTED, "%s: too many tiles", who);
   p.idesc = idesc_f8f6f4(g.w_fmt, g.x_fmt, g.w_kind == 1 ? 1 : 0, 0, kTkRows, 0);
-  // Weights that one token tile reads, and that fill more than half of L2, leave it first: they would only push out what
-  // the next kernels read (1 x 8192 x 28672: 41.5 -> 39.6 us; 40 rows over 64 experts of 7168 x 2048: 75 -> 71). Smaller ones may
-  // still be there at the next call (1 x 1024 x 16384, 16 MB: 9.3 us, and 10.0 if they leave first).
+  // Weights that one token tile reads, or the few token tiles of an expert side by side, and that fill more than half of L2,
+  // leave it first: they would only push out what the next kernels read (in turn on one GPU: 1 x 8192 x 28672 41.5 and
+  // 39.6 us, 40 rows over 64 experts of 7168 x 2048 75 and 71, two token tiles of 250 rows on an expert of 4096 x 28672 39.1 and
+  // 35.4; GPUs differ by as much).  Smaller ones may still be there at the next call (1 x 1024 x 16384, 16 MB: 9.3 us, and
+  // 10.0 if they leave first).
   const double weights = (moe ? std::max(1.0, active) : 1.0) * p.n_tiles * kTkRows * (double)p.K;
   p.l2_w = (moe || tok_tiles == 1) && weights > 64e6 ? 2 : 1;
   CUtensorMap tmX;

@@ -6,8 +6,8 @@
 // between the instructions of the selection, so that takes few.  Choices become order-preserving 32-bit keys.  The
 // (k + 2)-th largest of the 32 lanes' maxima (redux.sync) is a bound that at least k + 2 keys reach and few more; those
 // (almost always at most 32) are packed one to a lane in the order of their index, and each counts the better ones.  Where
-// more than 32 reach the bound the choices are taken one after the other instead.  What bounds the kernel is the integer
-// pipe, at half rate: comparisons and selections.
+// more than 32 reach the bound the choices are taken one after the other instead.  What bounds the kernel is how fast
+// instructions issue (16384 x 256: 78 % of the issue slots, the integer pipe 56 %, HBM 8 %): comparisons and selections.
 //
 // What is compared.  Without a bias s is monotone in the logit, so the logits themselves are the keys and the choice is
 // exact.  With a bias (and for sums of two) the keys are fp32 values of s + b.  s is off by at most err = 2^-20 (sigmoid) or
@@ -16,10 +16,10 @@
 // order a, b lie closer than 2 err + 2^-23 (|a| + |b|), or in which a group that goes may be off by as much as sets it
 // behind one that stays (2 err and 2^-24 of its two choices and of their sum, each), is settled in fp64: the groups alone (groups_exact), the candidates' order alone (rank_exact), or, where neither will do,
 // the whole choice (choose_exact).  It is right to fp64, at the speed of fp32 for nearly all rows (16384 tokens, 256
-// experts, k = 8: 34 rows needed it; settling them all by choose_exact took the kernel from 24 to 31 us).
+// experts, k = 8: the fp64 pipe is busy 0.007 % of the time; settling all doubtful rows by choose_exact took 7 us more).
 //
-// Measured, 16384 tokens, k = 8, 64 / 128 / 256 / 384 experts: softmax 9.8 / 10.6 / 12.2 / 13.6 us; sigmoid, bias, 8 groups by
-// their two largest 17 / 20 / 24 / 30 us.  8 tokens: 2.7 to 4.0 us, launch and latency.
+// Measured, 16384 tokens, k = 8, 64 / 128 / 256 / 384 experts: softmax 10.1 / 10.8 / 12.5 / 14.0 us; sigmoid, bias, 8 groups by
+// their two largest 18 / 21 / 26 / 32 us.  8 tokens: 2.8 to 4.5 us, launch and latency.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cfloat>

@@ -9,11 +9,11 @@
 //     counters, no atomics whose order matters: the same input gives the same order.
 // Row kernel: one CTA per token reads the row once (it stays in registers between the maximum and the cast) and stores
 // top_k copies, 16 bytes a thread.  Bound: HBM, tokens * cols * (4 or 2) bytes in and tokens * top_k * cols out: 8191 x 7168
-// bf16, top_k = 8 in 105 us (5.6 TB/s), of which the plan is 14, partly beside the rows.  16 tokens: 6.3 us.
+// bf16, top_k = 8 in 107 us (5.5 TB/s), of which the plan is 14, partly beside the rows.  16 tokens: 6.3 us.
 //
 // Combine reads the top_k rows of a token side by side (8 predicated 16-byte loads in flight per thread; with branches
 // around them the loads went out one by one and the same case took 272 us) and adds them in the order of the slots in
-// fp32.  Bound: HBM, 8191 x 7168, top_k = 8 with residual in 173 us; its gradients for 4095 tokens in 155 us.
+// fp32.  Bound: HBM, 8191 x 7168, top_k = 8 with residual in 175 us; its gradients for 4095 tokens in 161 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
