@@ -405,8 +405,9 @@ B2X_API b2x_status b2x_epilogue_backward(const void* grad, int64_t ld_grad, cons
  * remaining slots hold expert -1 and weight 0.  NaN ranks above all numbers
  * and its weight is NaN.  A row whose chosen s are all 0 in 64 bits (sigmoid of
  * logits below -709, such as the type's lowest value) has weights 0 also where
- * they are renormalized.  Weights are right to 25 x 2^-24 of their value, those
- * of a softmax over all experts to (21 + 3 ln(experts) + experts / 16) x 2^-24.
+ * they are renormalized.  Weights above 2^-126 are right to 25 x 2^-24 of their
+ * value, those of a softmax over all experts to (23 + 3 ln(experts) +
+ * experts / 16) x 2^-24.
  * experts <= 1024, top_k <= 32.
  */
 typedef struct {

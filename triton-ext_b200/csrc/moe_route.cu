@@ -11,12 +11,15 @@
 //
 // What is compared.  Without a bias s is monotone in the logit, so the logits themselves are the keys and the choice is
 // exact.  With a bias (and for sums of two) the keys are fp32 values of s + b.  s is off by at most err = 2^-20 (sigmoid) or
-// (2^-20 + (VPL + 5) 2^-24) max s: the approximate exponential and reciprocal together stay below 2^-20 relative and the
-// softmax's sum adds VPL + 5 roundings; s + b is rounded once, by 2^-24 of it.  A row in which two neighbours of the
+// (VPL + 31) 2^-24 max s.  In u = 2^-24, e^-d is off by (4 + 3 d) u of itself: 2^-22 of the instruction, the rest its
+// argument's roundings.  sigma: s (1 - s) (4 + 3 |l|) u < 2 u, the sum and the reciprocal 3 u.  Softmax: the largest by 4 u, the
+// sum by 4 u and 3 u of the mean distance from the maximum, at most 5 for 1024 experts (N of them at d: N d e^-d / (1 + N e^-d)),
+// quotient and product by 2 u, and VPL + 5 additions.  s + b is rounded once, by u of it.  A row in which two neighbours of the
 // order a, b lie closer than 2 err + 2^-23 (|a| + |b|), or in which a group that goes may be off by as much as sets it
-// behind one that stays (2 err and 2^-24 of its two choices and of their sum, each), is settled in fp64: the groups alone (groups_exact), the candidates' order alone (rank_exact), or, where neither will do,
-// the whole choice (choose_exact).  It is right to fp64, at the speed of fp32 for nearly all rows (16384 tokens, 256
-// experts, k = 8: the fp64 pipe is busy 0.007 % of the time; settling all doubtful rows by choose_exact took 7 us more).
+// behind one that stays (2 err and 2^-24 of its two choices and of their sum, each), is settled in fp64: the groups alone
+// (groups_exact), the candidates' order alone (rank_exact), or, where neither will do, the whole choice (choose_exact).  It is
+// right to fp64, at the speed of fp32 for nearly all rows (16384 tokens, 256 experts, k = 8, sigmoid: the fp64 pipe is busy
+// 0.007 % of the time; settling all doubtful rows by choose_exact took 7 us more).
 //
 // Measured, 16384 tokens, k = 8, 64 / 128 / 256 / 384 experts: softmax 10.1 / 10.8 / 12.5 / 14.0 us; sigmoid, bias, 8 groups by
 // their two largest 18 / 21 / 26 / 32 us.  8 tokens: 2.8 to 4.5 us, launch and latency.
@@ -391,7 +394,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 10 : (VPL <= 16 ?
   float err = 0.0f;
   if (values) {
     const float inv = p.sigmoid ? 0.0f : __fdiv_rn(1.0f, sum);  // also the largest s
-    err = p.sigmoid ? 0x1p-20f : (0x1p-20f + (VPL + 5) * 0x1p-24f) * inv;
+    err = p.sigmoid ? 0x1p-20f : (VPL + 31) * 0x1p-24f * inv;
     float b[VPL];
     if (p.bias) load_bias<VPL>(p, e0, b);
 #pragma unroll
@@ -671,7 +674,7 @@ __device__ __forceinline__ void store_logits(const RouteParams& p, int64_t row, 
 //   softmax:  dl_e = s_e (ds_e - sum_i s_i ds_i); renormalised, w / scale is the softmax p over the chosen ones and
 //             dl_e = scale p_e (d_e - sum_i p_i d_i), which needs the chosen logits alone.
 // The chosen ones are made as the weights are; the dense part takes the approximate exponential, which is within
-// (4 + 3 |l - max|) 2^-24 of s (16384 x 128: 7.0 us, with the library's 7.6).
+// (4 + 3 |l - max|) 2^-24 of s (16384 x 128: 6.9 us, with the library's 7.6).
 // An expert named in two slots gets the sum of both.  The rest of the row is the dense part (0 except for the
 // softmax over all experts), stored first; the chosen ones are stored over it after a __syncwarp.
 template <int VPL>
