@@ -12,8 +12,9 @@ the whole run can be captured into a CUDA graph.  All arithmetic happens in the 
 include/b2x.h); there is no CPU path.  The calls run on the current stream of their tensors' device and keep no state
 between them.
 
-A new result whose rows are no multiple of 8 values (16 of float8) is a view of rows padded to one: not contiguous.  float8 operands whose rows do not start on 16-byte boundaries are copied to padded rows in every call; a
-weight that is kept spares that where it is stored padded: torch.empty(N, -(-K // 16) * 16)[:, :K].
+A new result whose rows are no multiple of 8 values (16 of float8) is a view of rows padded to one: not contiguous.
+float8 operands whose rows do not start on 16-byte boundaries are copied to padded rows in every call; a weight that is
+kept spares that where it is stored padded: torch.empty(N, -(-K // 16) * 16)[:, :K].
 """
 from __future__ import annotations
 
